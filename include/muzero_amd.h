@@ -512,6 +512,31 @@ int mz_inference_x3_forward(const void *packed, const void *ends, const float *b
  * stamps, (ceil(n / 4), 32) int64 on the device (tools/restower_stamps.py reads them) */
 int mz_restower_x3_stamps(const void *packed, const float *bias, const float *x, float *y, int64_t n, void *stamps, void *stream);
 
+/* ------------------------------------------------------------------------------------------
+ * The global gradient norm and clipping by it (between main.py:266 loss.backward() and main.py:267 optimizer.step())
+ * ---------------------------------------------------------------------------------------- */
+/* one tensor of a list: n elements that lie together (any order of its axes), f32 / bf16 / f16; the LIST is a HOST array, read
+ * during the call.  dst is read by mz_grad_clip only: == src for scaling in place, otherwise memory of its own; its dtype is
+ * src's, or f32 (16-bit gradients into the f32 ones that the optimiser reads).  Tensors with n == 0 are passed over. */
+typedef struct mz_grad_tensor {
+    const void *src;
+    void *dst;
+    int64_t n;
+    int32_t src_dtype, dst_dtype;
+} mz_grad_tensor;
+
+/* norm = sqrt(sum over all tensors and elements of g^2), one f32 on the device.  Squares and sums are held in 64 bits, in a fixed
+ * order: two calls on the same data return the same bits.  An inf or NaN among the gradients makes the norm inf or NaN.
+ *   workspace : device scratch of >= mz_grad_workspace_bytes(count) bytes, 8-byte aligned; calls that overlap in time need one each */
+int64_t mz_grad_workspace_bytes(int32_t count);
+int mz_grad_norm(const mz_grad_tensor *tensors, int32_t count, void *workspace, int64_t workspace_bytes, float *norm, void *stream);
+/* the same, and dst = src * min(1, max_norm / (norm + 1e-6)) for every tensor, the factor rounded to f32 and each product once to dst's
+ * dtype.  max_norm >= 0; a norm below it leaves the values as they are (copied if dst is not src).  With an infinite norm the factor is 0
+ * (infinite gradients become NaN), with a NaN it is NaN: what the formula gives.  Outputs that overlap each other or another
+ * tensor's gradients are refused. */
+int mz_grad_clip(const mz_grad_tensor *tensors, int32_t count, double max_norm, void *workspace, int64_t workspace_bytes, float *norm,
+                 void *stream);
+
 #ifdef __cplusplus
 }
 #endif

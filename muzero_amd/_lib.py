@@ -119,6 +119,8 @@ SIGNATURES = {
     "mz_restower_x3_stamps": [_p, _p, _p, _p, _i64, _p, _p],
     "mz_tower_x3_pack_ends": [_p, _i32, _p, _p, _p],
     "mz_tower_x3_forward": [_p, _p, _p, _p, _p, _i32, _p, _p, _i64, _p],
+    "mz_grad_norm": [_p, _i32, _p, _i64, _p, _p],
+    "mz_grad_clip": [_p, _i32, C.c_double, _p, _i64, _p, _p],
     "mz_inference_x3_forward": [_p, _p, _p, _p, _p, _i32, C.POINTER(HeadsWeights), _p, _p, _p, _p, _i64, _p],
 }
 for _name, _args in SIGNATURES.items():
@@ -129,11 +131,13 @@ lib.mz_search_workspace_bytes.restype = C.c_int64
 lib.mz_search_workspace_bytes.argtypes = [_i32, _i32]
 lib.mz_conv3x3_wgrad_workspace.restype = C.c_int64
 lib.mz_conv3x3_wgrad_workspace.argtypes = [_i64]
+lib.mz_grad_workspace_bytes.restype = C.c_int64
+lib.mz_grad_workspace_bytes.argtypes = [_i32]
 lib.mz_last_error.restype = C.c_char_p
 lib.mz_last_error.argtypes = []
 lib.mz_version.restype = C.c_int
 lib.mz_version.argtypes = []
-EXPORTS = sorted(list(SIGNATURES) + ["mz_last_error", "mz_version", "mz_search_workspace_bytes", "mz_conv3x3_wgrad_workspace"])
+EXPORTS = sorted(list(SIGNATURES) + ["mz_last_error", "mz_version", "mz_search_workspace_bytes", "mz_conv3x3_wgrad_workspace", "mz_grad_workspace_bytes"])
 
 
 def call(name, *args):
