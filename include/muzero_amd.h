@@ -537,6 +537,35 @@ int mz_grad_norm(const mz_grad_tensor *tensors, int32_t count, void *workspace, 
 int mz_grad_clip(const mz_grad_tensor *tensors, int32_t count, double max_norm, void *workspace, int64_t workspace_bytes, float *norm,
                  void *stream);
 
+/* ------------------------------------------------------------------------------------------
+ * The policy's cross-entropy with its gradient (main.py:261-266: p_loss = mean of -sum pi log p, and its backward), from LOGITS
+ * ---------------------------------------------------------------------------------------- */
+/* Row i over the actions j that are legal, with m = max x, z = sum exp(x - m), T = sum t:
+ *     loss_i = w_i (T log z - sum t (x - m))                                 = -w_i sum t log softmax(x)
+ *     grad_i = grad_out w_i scale (T exp(x - m) / z - t), 0 where not legal
+ * A term with t = 0 counts as 0 also where x = -inf.  A row without a legal action above -inf, or with w_i = 0, gives loss 0 and
+ * gradient 0 whatever it holds; values at places that are not legal are never used.  NaN and +inf elsewhere make their row NaN.
+ * Softmax and row sums in f32, the sum over rows in 64 bits in a fixed order, gradients rounded once to the logits' dtype. */
+typedef struct mz_policy_loss_args {
+    const void *logits;         /* (n, v) of dtype, rows logits_stride elements apart */
+    const void *targets;        /* (n, v) of target_dtype (dtype, or MZ_F32), rows targets_stride apart */
+    const uint8_t *allowed;     /* (n, v) bytes, 0 = not legal, rows allowed_stride apart; NULL = all legal */
+    const uint64_t *board;      /* instead, v = 65: (n) masks of legal placements; action 64 is legal where the mask is 0 */
+    const float *weight;        /* (n) or NULL = 1 */
+    const float *grad_out;      /* the gradient of the loss: one value (stride 0) or one per row (1); NULL = 1 */
+    float *row_loss;            /* out (n): the loss_i, or NULL */
+    float *loss;                /* out: scale * sum of the loss_i, or NULL */
+    void *grad;                 /* out (n, v) of dtype, rows grad_stride apart, or NULL */
+    int64_t n, v;               /* n < 2^22, v <= 2^24 */
+    int64_t logits_stride, targets_stride, allowed_stride, grad_stride;
+    double scale;               /* 1 / n for a mean */
+    int32_t dtype, target_dtype, grad_out_stride;
+    int32_t skip_one;           /* with one grad_out and grad alone: leave grad as it is where grad_out is 1 */
+} mz_policy_loss_args;
+/* workspace: device scratch of >= mz_policy_loss_workspace_bytes(n, v) bytes, 16-byte aligned; calls that overlap in time need one each */
+int64_t mz_policy_loss_workspace_bytes(int64_t n, int64_t v);
+int mz_policy_loss(const mz_policy_loss_args *args, void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

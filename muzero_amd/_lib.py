@@ -62,6 +62,13 @@ class HeadsWeights(C.Structure):
     _fields_ = [(k, C.c_void_p) for k in ("pc_w", "pc_b", "p1_w", "p1_b", "p2_w", "p2_b", "vc_w", "vc_b", "v1_w", "v1_b")]
 
 
+class PolicyLossArgs(C.Structure):
+    """mz_policy_loss_args"""
+    _fields_ = ([(k, C.c_void_p) for k in ("logits", "targets", "allowed", "board", "weight", "grad_out", "row_loss", "loss", "grad")]
+                + [(k, C.c_int64) for k in ("n", "v", "logits_stride", "targets_stride", "allowed_stride", "grad_stride")]
+                + [("scale", C.c_double)] + [(k, C.c_int32) for k in ("dtype", "target_dtype", "grad_out_stride", "skip_one")])
+
+
 if not os.path.exists(LIB_PATH):
     raise ImportError(
         "muzero_amd: %s is missing. Build it with `make -C muzero_amd/csrc` (or "
@@ -119,6 +126,7 @@ SIGNATURES = {
     "mz_restower_x3_stamps": [_p, _p, _p, _p, _i64, _p, _p],
     "mz_tower_x3_pack_ends": [_p, _i32, _p, _p, _p],
     "mz_tower_x3_forward": [_p, _p, _p, _p, _p, _i32, _p, _p, _i64, _p],
+    "mz_policy_loss": [C.POINTER(PolicyLossArgs), _p, _i64, _p],
     "mz_grad_norm": [_p, _i32, _p, _i64, _p, _p],
     "mz_grad_clip": [_p, _i32, C.c_double, _p, _i64, _p, _p],
     "mz_inference_x3_forward": [_p, _p, _p, _p, _p, _i32, C.POINTER(HeadsWeights), _p, _p, _p, _p, _i64, _p],
@@ -131,13 +139,16 @@ lib.mz_search_workspace_bytes.restype = C.c_int64
 lib.mz_search_workspace_bytes.argtypes = [_i32, _i32]
 lib.mz_conv3x3_wgrad_workspace.restype = C.c_int64
 lib.mz_conv3x3_wgrad_workspace.argtypes = [_i64]
+lib.mz_policy_loss_workspace_bytes.restype = C.c_int64
+lib.mz_policy_loss_workspace_bytes.argtypes = [_i64, _i64]
 lib.mz_grad_workspace_bytes.restype = C.c_int64
 lib.mz_grad_workspace_bytes.argtypes = [_i32]
 lib.mz_last_error.restype = C.c_char_p
 lib.mz_last_error.argtypes = []
 lib.mz_version.restype = C.c_int
 lib.mz_version.argtypes = []
-EXPORTS = sorted(list(SIGNATURES) + ["mz_last_error", "mz_version", "mz_search_workspace_bytes", "mz_conv3x3_wgrad_workspace", "mz_grad_workspace_bytes"])
+EXPORTS = sorted(list(SIGNATURES) + ["mz_last_error", "mz_version", "mz_search_workspace_bytes", "mz_conv3x3_wgrad_workspace", "mz_grad_workspace_bytes",
+                                      "mz_policy_loss_workspace_bytes"])
 
 
 def call(name, *args):

@@ -1,0 +1,127 @@
+"""What is done with a policy's logits: learning from target distributions (the cross-entropy of main.py:261 with the gradient that
+main.py:266 asks autograd for), on the hand-written kernels of muzero_amd/csrc/policy_*.hip.
+
+The network's ``Prediction`` returns softmaxed probabilities; these operators take what stands before that softmax (or the
+logarithm of the probabilities, which differs from it by a constant per row).  Rows are games, positions or requests; the columns
+are actions: this game's 65 or any other number.  ``legal`` says which of them may be played: a bool tensor of the logits' shape, or
+for 65 actions the (n,) int64 bitboards that ``BatchedEnv.legal`` holds (the pass is legal where no square is).  No CPU fallback:
+host tensors raise."""
+import ctypes as C
+
+import torch
+
+from . import _lib as L
+
+_DT = {torch.float32: L.MZ_F32, torch.bfloat16: L.MZ_BF16, torch.float16: L.MZ_F16}
+
+
+def _rows(who, name, t, shape=None, dtypes=tuple(_DT)):
+    """(n, v) on the GPU whose rows hold their elements together; returns the rows' stride"""
+    if not t.is_cuda:
+        raise L.MzError("%s: muzero_amd kernels need device tensors; got %s on %s (no CPU fallback)" % (who, name, t.device))
+    if t.dim() != 2 or t.dtype not in dtypes:
+        raise L.MzError("%s: %s has to be (n, actions) of %s, got %s %s" % (who, name, " / ".join(str(d) for d in dtypes), tuple(t.shape), t.dtype))
+    if shape is not None and t.shape != shape:
+        raise L.MzError("%s: %s has shape %s, the logits have %s" % (who, name, tuple(t.shape), tuple(shape)))
+    if t.shape[1] < 1:
+        raise L.MzError("%s: needs at least one action" % who)
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        raise L.MzError("%s: the actions of a row of %s have to lie together, got strides %s" % (who, name, t.stride()))
+    return t.stride(0)
+
+
+def _per_row(who, name, t, n, dtype, dev):
+    if not t.is_cuda or t.dtype != dtype or tuple(t.shape) != (n,) or not t.is_contiguous() or t.device != dev:
+        raise L.MzError("%s: %s has to be a contiguous %s tensor of shape (%d,) on %s, got %s %s on %s" % (who, name, dtype, n, dev, tuple(t.shape), t.dtype, t.device))
+    return t.data_ptr()
+
+
+def _legal(who, legal, logits):
+    """-> (pointer of the bytes, their row stride, pointer of the bitboards)"""
+    if legal is None:
+        return None, 0, None
+    if legal.device != logits.device:
+        raise L.MzError("%s: legal has to be on the logits' device, got %s (no CPU fallback)" % (who, legal.device))
+    if legal.dtype == torch.int64:
+        if logits.shape[1] != 65:
+            raise L.MzError("%s: bitboards go with 65 actions, the logits have %d" % (who, logits.shape[1]))
+        return None, 0, _per_row(who, "legal", legal, logits.shape[0], torch.int64, logits.device)
+    return legal.data_ptr(), _rows(who, "legal", legal, logits.shape, (torch.bool,)), None
+
+
+def _loss_call(logits, targets, weight, legal, scale, go=None, go_stride=0, row_loss=None, loss=None, grad=None, skip_one=0):
+    """mz_policy_loss on tensors that _CrossEntropy has checked"""
+    n, v = logits.shape
+    dev = logits.device
+    allowed, allowed_stride, board = _legal("cross_entropy", legal, logits)
+    ptr = lambda t: None if t is None else t.data_ptr()   # noqa: E731
+    a = L.PolicyLossArgs(logits.data_ptr(), targets.data_ptr(), allowed, board, ptr(weight), ptr(go), ptr(row_loss), ptr(loss), ptr(grad), n, v,
+                         logits.stride(0), targets.stride(0), allowed_stride, v, scale, _DT[logits.dtype], _DT[targets.dtype], go_stride, skip_one)
+    nbytes = L.lib.mz_policy_loss_workspace_bytes(n, v)
+    if nbytes < 0:
+        raise L.MzError("cross_entropy: (n, actions) = (%d, %d) is too large" % (n, v))
+    with torch.cuda.device(dev):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        L.call("mz_policy_loss", C.byref(a), ws.data_ptr(), nbytes, L.current_stream())
+
+
+class _CrossEntropy(torch.autograd.Function):
+    """The gradient comes out of the forward pass over the rows, for a loss whose own gradient is 1 (what loss.backward() starts
+    from).  backward launches the same kernel with the gradient it is given: where that is 1 the kernel leaves at once, otherwise it
+    computes the rows again, so a scaled 16-bit gradient is rounded once, after the scale."""
+
+    @staticmethod
+    def forward(ctx, logits, targets, weight, legal, reduction):
+        n, v = logits.shape
+        need = ctx.needs_input_grad[0]
+        scale = 1.0 / n if reduction == "mean" and n else 1.0
+        ctx.reduction, ctx.scale, ctx.ready = reduction, scale, None
+        if need:
+            ctx.save_for_backward(logits, targets, weight, legal)
+        if n == 0:
+            return logits.new_full((0,) if reduction == "none" else (), float("nan") if reduction == "mean" else 0.0, dtype=torch.float32)
+        if reduction == "none":
+            rows = torch.empty(n, dtype=torch.float32, device=logits.device)
+            _loss_call(logits, targets, weight, legal, scale, row_loss=rows)
+            return rows
+        loss = torch.empty((), dtype=torch.float32, device=logits.device)
+        if need:
+            ctx.ready = torch.empty((n, v), dtype=logits.dtype, device=logits.device)
+        _loss_call(logits, targets, weight, legal, scale, loss=loss, grad=ctx.ready)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, go):
+        logits, targets, weight, legal = ctx.saved_tensors
+        grad, ctx.ready = ctx.ready, None      # handed out once; a second backward pass gets memory of its own
+        skip = grad is not None
+        if grad is None:
+            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        if logits.shape[0]:
+            go = go.contiguous()
+            _loss_call(logits, targets, weight, legal, ctx.scale, go=go, go_stride=int(ctx.reduction == "none"), grad=grad, skip_one=int(skip))
+        return grad, None, None, None, None
+
+
+def cross_entropy(logits, targets, weight=None, legal=None, reduction="mean"):
+    """-sum over the legal actions of targets * log softmax(logits), per row times `weight`: the mean over the n rows, their "sum", or
+    "none" = the (n,) rows, in float32, differentiable in the logits.
+
+    logits (n, v) float32 / bfloat16 / float16; targets (n, v) of the same dtype or float32, any non-negative shares (they need not add
+    up to 1); rows may be strided, a row's elements lie together.  weight float32 (n,): a row of weight 0 (padding) counts in the mean's n
+    but gives no loss and no gradient, whatever it holds.  legal: see the module; other places are never used, their gradient is 0,
+    and a row without a legal action gives 0.  Targets of 0 count as 0 also against a logit of -inf."""
+    who = "cross_entropy"
+    _rows(who, "logits", logits)
+    _rows(who, "targets", targets, logits.shape, (logits.dtype,) if logits.dtype == torch.float32 else (logits.dtype, torch.float32))
+    if targets.device != logits.device:
+        raise L.MzError("%s: targets are on %s, the logits on %s" % (who, targets.device, logits.device))
+    if targets.requires_grad or (weight is not None and weight.requires_grad):
+        raise L.MzError("%s: targets and weights carry no gradient (detach them)" % who)
+    if weight is not None:
+        _per_row(who, "weight", weight, logits.shape[0], torch.float32, logits.device)
+    _legal(who, legal, logits)
+    if reduction not in ("mean", "sum", "none"):
+        raise L.MzError("%s: reduction is 'mean', 'sum' or 'none', got %r" % (who, reduction))
+    return _CrossEntropy.apply(logits, targets, weight, legal, reduction)
