@@ -566,6 +566,39 @@ typedef struct mz_policy_loss_args {
 int64_t mz_policy_loss_workspace_bytes(int64_t n, int64_t v);
 int mz_policy_loss(const mz_policy_loss_args *args, void *workspace, int64_t workspace_bytes, void *stream);
 
+/* ------------------------------------------------------------------------------------------
+ * One action per row from a policy's LOGITS (beside mz_select_action and mz_softmax_sample, which draw from visit counts)
+ * ---------------------------------------------------------------------------------------- */
+/* Row i with one given uniform u in [0, 1), over the actions that are legal and whose logit is above -inf, m = max x:
+ *   temperature T = 0 : the action of the largest logit, the lowest index of equals
+ *   T > 0             : w_j = exp((x_j - m) / T); the actions in the order (x descending, index ascending);
+ *     top_k > 0       : the first k of them (0, or k >= v: all)
+ *     top_p < 1       : of these, the ones before which less than top_p times their total mass lies
+ *     min_p > 0       : of these, the ones with w_j >= min_p
+ *     the first of the order always stays; with R the mass of what stays, the answer is the lowest index j with
+ *     sum over kept i <= j of w_i > u R   (the last kept action if rounding, or u >= 1, leaves none).
+ * Masses in 64 bits, in an order that does not change between calls.  A row without a legal action above -inf, with a NaN or +inf
+ * at a legal place, or with a NaN or infinite temperature answers -1.  Values at places that are not legal are never used. */
+typedef struct mz_sample_args {
+    const void *logits;             /* (n, v) of dtype, rows logits_stride elements apart */
+    const uint8_t *allowed;         /* (n, v) bytes, 0 = not legal, rows allowed_stride apart; NULL = all legal */
+    const uint64_t *board;          /* instead, v = 65: (n) masks of legal placements; action 64 is legal where the mask is 0 */
+    const double *u;                /* (n) */
+    const float *temperature_of;    /* (n), or NULL = temperature for all rows; a value <= 0 counts as 0 */
+    const int32_t *top_k_of;        /* (n), or NULL = top_k; a value <= 0 is off */
+    const float *top_p_of;          /* (n), or NULL = top_p; a value >= 1 is off, one below 0 counts as 0 */
+    const float *min_p_of;          /* (n), or NULL = min_p; a value <= 0 is off, one above 1 counts as 1 */
+    int32_t *action;                /* out (n) */
+    int64_t n, v;                   /* n < 2^22, v <= 2^19 */
+    int64_t logits_stride, allowed_stride, top_k;
+    double temperature, top_p, min_p;
+    int32_t dtype;
+} mz_sample_args;
+/* workspace: device scratch of >= mz_sample_actions_workspace_bytes(n, v) bytes (0: none needed), 8-byte aligned; calls that overlap in
+ * time need one each */
+int64_t mz_sample_actions_workspace_bytes(int64_t n, int64_t v);
+int mz_sample_actions(const mz_sample_args *args, void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

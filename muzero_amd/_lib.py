@@ -69,6 +69,13 @@ class PolicyLossArgs(C.Structure):
                 + [("scale", C.c_double)] + [(k, C.c_int32) for k in ("dtype", "target_dtype", "grad_out_stride", "skip_one")])
 
 
+class SampleArgs(C.Structure):
+    """mz_sample_args"""
+    _fields_ = ([(k, C.c_void_p) for k in ("logits", "allowed", "board", "u", "temperature_of", "top_k_of", "top_p_of", "min_p_of", "action")]
+                + [(k, C.c_int64) for k in ("n", "v", "logits_stride", "allowed_stride", "top_k")]
+                + [(k, C.c_double) for k in ("temperature", "top_p", "min_p")] + [("dtype", C.c_int32)])
+
+
 if not os.path.exists(LIB_PATH):
     raise ImportError(
         "muzero_amd: %s is missing. Build it with `make -C muzero_amd/csrc` (or "
@@ -126,6 +133,7 @@ SIGNATURES = {
     "mz_restower_x3_stamps": [_p, _p, _p, _p, _i64, _p, _p],
     "mz_tower_x3_pack_ends": [_p, _i32, _p, _p, _p],
     "mz_tower_x3_forward": [_p, _p, _p, _p, _p, _i32, _p, _p, _i64, _p],
+    "mz_sample_actions": [C.POINTER(SampleArgs), _p, _i64, _p],
     "mz_policy_loss": [C.POINTER(PolicyLossArgs), _p, _i64, _p],
     "mz_grad_norm": [_p, _i32, _p, _i64, _p, _p],
     "mz_grad_clip": [_p, _i32, C.c_double, _p, _i64, _p, _p],
@@ -139,6 +147,8 @@ lib.mz_search_workspace_bytes.restype = C.c_int64
 lib.mz_search_workspace_bytes.argtypes = [_i32, _i32]
 lib.mz_conv3x3_wgrad_workspace.restype = C.c_int64
 lib.mz_conv3x3_wgrad_workspace.argtypes = [_i64]
+lib.mz_sample_actions_workspace_bytes.restype = C.c_int64
+lib.mz_sample_actions_workspace_bytes.argtypes = [_i64, _i64]
 lib.mz_policy_loss_workspace_bytes.restype = C.c_int64
 lib.mz_policy_loss_workspace_bytes.argtypes = [_i64, _i64]
 lib.mz_grad_workspace_bytes.restype = C.c_int64
@@ -148,7 +158,7 @@ lib.mz_last_error.argtypes = []
 lib.mz_version.restype = C.c_int
 lib.mz_version.argtypes = []
 EXPORTS = sorted(list(SIGNATURES) + ["mz_last_error", "mz_version", "mz_search_workspace_bytes", "mz_conv3x3_wgrad_workspace", "mz_grad_workspace_bytes",
-                                      "mz_policy_loss_workspace_bytes"])
+                                      "mz_policy_loss_workspace_bytes", "mz_sample_actions_workspace_bytes"])
 
 
 def call(name, *args):

@@ -1,5 +1,6 @@
-"""What is done with a policy's logits: learning from target distributions (the cross-entropy of main.py:261 with the gradient that
-main.py:266 asks autograd for), on the hand-written kernels of muzero_amd/csrc/policy_*.hip.
+"""What is done with a policy's logits: drawing an action (beside ``mcts.select_action`` and ``arena.softmax_sample``, which draw
+from visit counts, main.py:128-140, test.py:228-243) and learning from target distributions (the cross-entropy of main.py:261 with the
+gradient that main.py:266 asks autograd for), on the hand-written kernels of muzero_amd/csrc/policy_*.hip.
 
 The network's ``Prediction`` returns softmaxed probabilities; these operators take what stands before that softmax (or the
 logarithm of the probabilities, which differs from it by a constant per row).  Rows are games, positions or requests; the columns
@@ -125,3 +126,50 @@ def cross_entropy(logits, targets, weight=None, legal=None, reduction="mean"):
     if reduction not in ("mean", "sum", "none"):
         raise L.MzError("%s: reduction is 'mean', 'sum' or 'none', got %r" % (who, reduction))
     return _CrossEntropy.apply(logits, targets, weight, legal, reduction)
+
+
+def _setting(who, name, value, n, dtype, dev, ok):
+    """-> (pointer of one value per row, the one value of all rows)"""
+    if torch.is_tensor(value):
+        return _per_row(who, name, value, n, dtype, dev), 0
+    if not ok(value):
+        raise L.MzError("%s: %s = %r is out of its range" % (who, name, value))
+    return None, value
+
+
+def sample_actions(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, legal=None, out=None):
+    """One action per row of logits (n, actions), drawn with the given uniforms u (float64 (n,) in [0, 1)): int32 (n,).
+
+    The draw is from softmax(logits / temperature) over the legal actions, cut to the top_k most likely (0 = all), of these to the
+    fewest most likely that together reach the share top_p, of these to the ones at least min_p times as likely as the best; equal
+    logits go to the lower index, the best action always stays, temperature 0 takes it.  The answer is the lowest index at which the
+    kept mass, cumulated in the order of the indices, exceeds u times its total.  Every setting is a number, or a tensor with one value
+    per row (float32; top_k int32).  Masses are held in 64 bits in a fixed order: the same call gives the same actions.
+
+    logits float32 / bfloat16 / float16, up to 2^19 actions, rows may be strided; legal: see the module.  A row without a legal action
+    (all others -inf count as not legal), with NaN or +inf at a legal place, or with a NaN or infinite temperature gives -1.  out: int32
+    (n,) to write into."""
+    who = "sample_actions"
+    logits = logits.detach()
+    stride = _rows(who, "logits", logits)
+    n, v = logits.shape
+    dev = logits.device
+    allowed, allowed_stride, board = _legal(who, legal, logits)
+    temperature_of, temperature = _setting(who, "temperature", temperature, n, torch.float32, dev, lambda x: x == 0 or 1e-30 <= x <= 1e30)
+    top_k_of, top_k = _setting(who, "top_k", top_k, n, torch.int32, dev, lambda x: x == int(x) and 0 <= x < 1 << 62)
+    top_p_of, top_p = _setting(who, "top_p", top_p, n, torch.float32, dev, lambda x: 0 <= x <= 1)
+    min_p_of, min_p = _setting(who, "min_p", min_p, n, torch.float32, dev, lambda x: 0 <= x <= 1)
+    u_ptr = _per_row(who, "u", u, n, torch.float64, dev)
+    nbytes = L.lib.mz_sample_actions_workspace_bytes(n, v)
+    if nbytes < 0:
+        raise L.MzError("%s: (n, actions) = (%d, %d) is too large" % (who, n, v))
+    with torch.cuda.device(dev):
+        if out is None:
+            out = torch.empty(n, dtype=torch.int32, device=dev)
+        else:
+            _per_row(who, "out", out, n, torch.int32, dev)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        a = L.SampleArgs(logits.data_ptr(), allowed, board, u_ptr, temperature_of, top_k_of, top_p_of, min_p_of, out.data_ptr(), n, v, stride, allowed_stride,
+                         int(top_k), float(temperature), float(top_p), float(min_p), _DT[logits.dtype])
+        L.call("mz_sample_actions", C.byref(a), ws.data_ptr(), nbytes, L.current_stream())
+    return out

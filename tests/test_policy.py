@@ -50,3 +50,51 @@ def test_policy_loss_workspace_is_checked():
     with pytest.raises(L.MzError, match="null arguments"):
         L.call("mz_policy_loss", None, 1 << 40, 1 << 30, None)
     L.call("mz_policy_loss", C.byref(_args(L, n=0, logits=None, targets=None)), None, 0, None)   # no rows: nothing to do
+
+
+def test_sample_actions_refuses_host_tensors():
+    from muzero_amd import _lib as L
+    from muzero_amd import policy
+    with pytest.raises(L.MzError, match="no CPU fallback"):
+        policy.sample_actions(torch.zeros(2, 65), torch.zeros(2, dtype=torch.float64))
+
+
+def _sample(L, **kw):
+    P = 1 << 40                                   # never read: every call below is refused on the host
+    d = dict(logits=P, u=P, action=P, n=4, v=1000, logits_stride=1000, temperature=1.0, top_p=1.0)
+    d.update(kw)
+    a = L.SampleArgs()
+    for k, v in d.items():
+        setattr(a, k, v)
+    return a
+
+
+NAN = float("nan")
+
+
+@pytest.mark.parametrize("kw, why", [
+    (dict(n=-1), "n has to be"), (dict(n=1 << 22), "n has to be"), (dict(v=0), "v has to be"), (dict(v=(1 << 19) + 1), "v has to be"), (dict(dtype=3), "unknown dtype"),
+    (dict(v=64, board=1 << 40), "needs v = 65"), (dict(board=1 << 40, v=65, allowed=1 << 40), "not both"), (dict(temperature=-1.0), "temperature"),
+    (dict(temperature=NAN), "temperature"), (dict(temperature=1e-31), "temperature"), (dict(temperature=float("inf")), "temperature"), (dict(top_k=-1), "top_k"),
+    (dict(top_p=-0.1), "top_p"), (dict(top_p=1.1), "top_p"), (dict(top_p=NAN), "top_p"), (dict(min_p=-0.1), "min_p"), (dict(min_p=1.1), "min_p"), (dict(min_p=NAN), "min_p"),
+    (dict(logits=None), "null"), (dict(u=None), "null"), (dict(action=None), "null"), (dict(logits=(1 << 40) + 2), "misaligned"), (dict(logits_stride=-1), "negative"),
+    (dict(allowed=1 << 40, allowed_stride=-1), "negative"),
+])
+def test_sample_arguments_are_checked_before_any_launch(kw, why):
+    from muzero_amd import _lib as L
+    with pytest.raises(L.MzError, match=why):
+        L.call("mz_sample_actions", C.byref(_sample(L, **kw)), 1 << 40, 1 << 30, None)
+
+
+def test_sample_workspace_is_checked():
+    from muzero_amd import _lib as L
+    size = L.lib.mz_sample_actions_workspace_bytes
+    assert size(4, 512) == 0 and size(4, 513) == 4 * 5 * 12
+    for bad in ((-1, 65), (4, 0), (4, (1 << 19) + 1), (1 << 22, 65)):
+        assert size(*bad) == -1
+    for ws, nbytes, why in ((None, 1 << 30, "workspace"), ((1 << 40) + 4, 1 << 30, "misaligned"), (1 << 40, size(4, 1000) - 1, "needed")):
+        with pytest.raises(L.MzError, match=why):
+            L.call("mz_sample_actions", C.byref(_sample(L)), ws, nbytes, None)
+    with pytest.raises(L.MzError, match="null arguments"):
+        L.call("mz_sample_actions", None, 1 << 40, 1 << 30, None)
+    L.call("mz_sample_actions", C.byref(_sample(L, n=0, logits=None, u=None, action=None)), None, 0, None)   # no rows: nothing to do
