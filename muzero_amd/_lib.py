@@ -167,6 +167,16 @@ def call(name, *args):
         raise MzError("%s failed (%d): %s" % (name, rc, lib.mz_last_error().decode()))
 
 
+def call_on(index, name, *args):
+    """call on the current stream of GPU `index`, which need not be the current device; the stream is the entry point's last argument"""
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return call_on(index, name, *args)
+    rc = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        raise MzError("%s failed (%d): %s" % (name, rc, lib.mz_last_error().decode()))
+
+
 def current_stream():
     import torch
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)

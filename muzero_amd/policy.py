@@ -26,13 +26,14 @@ def _rows(who, name, t, shape=None, dtypes=tuple(_DT)):
         raise L.MzError("%s: %s has shape %s, the logits have %s" % (who, name, tuple(t.shape), tuple(shape)))
     if t.shape[1] < 1:
         raise L.MzError("%s: needs at least one action" % who)
-    if t.stride(1) != 1 and t.shape[1] > 1:
+    stride, step = t.stride()
+    if step != 1 and t.shape[1] > 1:
         raise L.MzError("%s: the actions of a row of %s have to lie together, got strides %s" % (who, name, t.stride()))
-    return t.stride(0)
+    return stride
 
 
 def _per_row(who, name, t, n, dtype, dev):
-    if not t.is_cuda or t.dtype != dtype or tuple(t.shape) != (n,) or not t.is_contiguous() or t.device != dev:
+    if not t.is_cuda or t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or t.device != dev:
         raise L.MzError("%s: %s has to be a contiguous %s tensor of shape (%d,) on %s, got %s %s on %s" % (who, name, dtype, n, dev, tuple(t.shape), t.dtype, t.device))
     return t.data_ptr()
 
@@ -50,59 +51,60 @@ def _legal(who, legal, logits):
     return legal.data_ptr(), _rows(who, "legal", legal, logits.shape, (torch.bool,)), None
 
 
-def _loss_call(logits, targets, weight, legal, scale, go=None, go_stride=0, row_loss=None, loss=None, grad=None, skip_one=0):
-    """mz_policy_loss on tensors that _CrossEntropy has checked"""
-    n, v = logits.shape
-    dev = logits.device
-    allowed, allowed_stride, board = _legal("cross_entropy", legal, logits)
-    ptr = lambda t: None if t is None else t.data_ptr()   # noqa: E731
-    a = L.PolicyLossArgs(logits.data_ptr(), targets.data_ptr(), allowed, board, ptr(weight), ptr(go), ptr(row_loss), ptr(loss), ptr(grad), n, v,
-                         logits.stride(0), targets.stride(0), allowed_stride, v, scale, _DT[logits.dtype], _DT[targets.dtype], go_stride, skip_one)
-    nbytes = L.lib.mz_policy_loss_workspace_bytes(n, v)
-    if nbytes < 0:
-        raise L.MzError("cross_entropy: (n, actions) = (%d, %d) is too large" % (n, v))
-    with torch.cuda.device(dev):
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        L.call("mz_policy_loss", C.byref(a), ws.data_ptr(), nbytes, L.current_stream())
-
-
 class _CrossEntropy(torch.autograd.Function):
     """The gradient comes out of the forward pass over the rows, for a loss whose own gradient is 1 (what loss.backward() starts
     from).  backward launches the same kernel with the gradient it is given: where that is 1 the kernel leaves at once, otherwise it
     computes the rows again, so a scaled 16-bit gradient is rounded once, after the scale."""
 
     @staticmethod
-    def forward(ctx, logits, targets, weight, legal, reduction):
-        n, v = logits.shape
+    def forward(ctx, logits, targets, weight, legal, reduction, args):
+        n = args.n
+        dev = logits.device
         need = ctx.needs_input_grad[0]
-        scale = 1.0 / n if reduction == "mean" and n else 1.0
-        ctx.reduction, ctx.scale, ctx.ready = reduction, scale, None
+        out = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32, device=dev)
         if need:
             ctx.save_for_backward(logits, targets, weight, legal)
-        if n == 0:
-            return logits.new_full((0,) if reduction == "none" else (), float("nan") if reduction == "mean" else 0.0, dtype=torch.float32)
+        ctx.args = args
+        ctx.ready = None
         if reduction == "none":
-            rows = torch.empty(n, dtype=torch.float32, device=logits.device)
-            _loss_call(logits, targets, weight, legal, scale, row_loss=rows)
-            return rows
-        loss = torch.empty((), dtype=torch.float32, device=logits.device)
-        if need:
-            ctx.ready = torch.empty((n, v), dtype=logits.dtype, device=logits.device)
-        _loss_call(logits, targets, weight, legal, scale, loss=loss, grad=ctx.ready)
-        return loss
+            args.row_loss = out.data_ptr()
+        else:
+            args.loss = out.data_ptr()
+            if need:
+                ctx.ready = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+                args.grad = ctx.ready.data_ptr()
+        nbytes = L.lib.mz_policy_loss_workspace_bytes(n, args.v)
+        if nbytes < 0:
+            raise L.MzError("cross_entropy: (n, actions) = (%d, %d) is too large" % (n, args.v))
+        if n == 0:
+            return out.fill_(float("nan") if reduction == "mean" else 0.0)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        L.call_on(dev.index, "mz_policy_loss", C.byref(args), ws.data_ptr(), nbytes)
+        return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, go):
-        logits, targets, weight, legal = ctx.saved_tensors
-        grad, ctx.ready = ctx.ready, None      # handed out once; a second backward pass gets memory of its own
-        skip = grad is not None
+        if torch.is_grad_enabled():            # create_graph: a second derivative is refused when it is asked for
+            return _backward_once(ctx, go)
+        logits = ctx.saved_tensors[0]          # also says if one of them was changed in place
+        args, grad = ctx.args, ctx.ready
+        ctx.ready = None                       # handed out once; a second backward pass gets memory of its own
+        args.skip_one = grad is not None
         if grad is None:
             grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        if logits.shape[0]:
+        if args.n:
             go = go.contiguous()
-            _loss_call(logits, targets, weight, legal, ctx.scale, go=go, go_stride=int(ctx.reduction == "none"), grad=grad, skip_one=int(skip))
-        return grad, None, None, None, None
+            args.grad, args.grad_out, args.grad_out_stride = grad.data_ptr(), go.data_ptr(), go.dim()
+            args.row_loss = args.loss = None
+            nbytes = L.lib.mz_policy_loss_workspace_bytes(args.n, args.v)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=grad.device)   # not the forward's: a captured backward keeps its own
+            L.call_on(grad.get_device(), "mz_policy_loss", C.byref(args), ws.data_ptr(), nbytes)
+        return grad, None, None, None, None, None
+
+
+@torch.autograd.function.once_differentiable
+def _backward_once(ctx, go):
+    return _CrossEntropy.backward(ctx, go)
 
 
 def cross_entropy(logits, targets, weight=None, legal=None, reduction="mean"):
@@ -114,18 +116,21 @@ def cross_entropy(logits, targets, weight=None, legal=None, reduction="mean"):
     but gives no loss and no gradient, whatever it holds.  legal: see the module; other places are never used, their gradient is 0,
     and a row without a legal action gives 0.  Targets of 0 count as 0 also against a logit of -inf."""
     who = "cross_entropy"
-    _rows(who, "logits", logits)
-    _rows(who, "targets", targets, logits.shape, (logits.dtype,) if logits.dtype == torch.float32 else (logits.dtype, torch.float32))
+    stride = _rows(who, "logits", logits)
+    dtype = logits.dtype
+    targets_stride = _rows(who, "targets", targets, logits.shape, (dtype, torch.float32))
     if targets.device != logits.device:
         raise L.MzError("%s: targets are on %s, the logits on %s" % (who, targets.device, logits.device))
     if targets.requires_grad or (weight is not None and weight.requires_grad):
         raise L.MzError("%s: targets and weights carry no gradient (detach them)" % who)
-    if weight is not None:
-        _per_row(who, "weight", weight, logits.shape[0], torch.float32, logits.device)
-    _legal(who, legal, logits)
+    n, v = logits.shape
+    weight_ptr = None if weight is None else _per_row(who, "weight", weight, n, torch.float32, logits.device)
+    allowed, allowed_stride, board = _legal(who, legal, logits)
     if reduction not in ("mean", "sum", "none"):
         raise L.MzError("%s: reduction is 'mean', 'sum' or 'none', got %r" % (who, reduction))
-    return _CrossEntropy.apply(logits, targets, weight, legal, reduction)
+    args = L.PolicyLossArgs(logits.data_ptr(), targets.data_ptr(), allowed, board, weight_ptr, None, None, None, None, n, v, stride, targets_stride, allowed_stride, v,
+                            1.0 / n if reduction == "mean" and n else 1.0, _DT[dtype], _DT[targets.dtype], 0, 0)
+    return _CrossEntropy.apply(logits, targets, weight, legal, reduction, args)
 
 
 def _setting(who, name, value, n, dtype, dev, ok):
@@ -150,7 +155,6 @@ def sample_actions(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, le
     (all others -inf count as not legal), with NaN or +inf at a legal place, or with a NaN or infinite temperature gives -1.  out: int32
     (n,) to write into."""
     who = "sample_actions"
-    logits = logits.detach()
     stride = _rows(who, "logits", logits)
     n, v = logits.shape
     dev = logits.device
@@ -163,13 +167,12 @@ def sample_actions(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, le
     nbytes = L.lib.mz_sample_actions_workspace_bytes(n, v)
     if nbytes < 0:
         raise L.MzError("%s: (n, actions) = (%d, %d) is too large" % (who, n, v))
-    with torch.cuda.device(dev):
-        if out is None:
-            out = torch.empty(n, dtype=torch.int32, device=dev)
-        else:
-            _per_row(who, "out", out, n, torch.int32, dev)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        a = L.SampleArgs(logits.data_ptr(), allowed, board, u_ptr, temperature_of, top_k_of, top_p_of, min_p_of, out.data_ptr(), n, v, stride, allowed_stride,
-                         int(top_k), float(temperature), float(top_p), float(min_p), _DT[logits.dtype])
-        L.call("mz_sample_actions", C.byref(a), ws.data_ptr(), nbytes, L.current_stream())
+    if out is None:
+        out = torch.empty(n, dtype=torch.int32, device=dev)
+    else:
+        _per_row(who, "out", out, n, torch.int32, dev)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    a = L.SampleArgs(logits.data_ptr(), allowed, board, u_ptr, temperature_of, top_k_of, top_p_of, min_p_of, out.data_ptr(), n, v, stride, allowed_stride,
+                     int(top_k), float(temperature), float(top_p), float(min_p), _DT[logits.dtype])
+    L.call_on(dev.index, "mz_sample_actions", C.byref(a), None if ws is None else ws.data_ptr(), nbytes)
     return out
