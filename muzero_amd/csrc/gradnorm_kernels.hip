@@ -35,26 +35,33 @@ __device__ __forceinline__ int tensor_of(const GradList &L, uint32_t c) {
     return __builtin_amdgcn_readfirstlane(k - 1);
 }
 
+// U vectors of 16 bytes per lane; a tensor's last chunk keeps whole vectors too, so that all of its loads are in flight together, and one element a
+// lane behind them
 template <int DT, int U> __device__ __forceinline__ double square_sum(const void *src, int64_t at, int64_t left) {
     constexpr int VEC = Elem<DT>::VEC;
     double acc = 0.0;
+    Words<DT, VEC> p[U];
     if (left >= (int64_t)U * 256 * VEC) {
-        Pack<typename Elem<DT>::T, VEC> p[U];
 #pragma unroll
-        for (int k = 0; k < U; ++k) p[k] = load_pack<DT, VEC>(src, at + ((int64_t)k * 256 + threadIdx.x) * VEC);
-#pragma unroll
-        for (int k = 0; k < U; ++k)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const double g = (double)Elem<DT>::up(p[k].v[j]);
-                acc = fma(g, g, acc);
-            }
+        for (int k = 0; k < U; ++k) p[k] = load_words<DT, VEC>(src, at + ((int64_t)k * 256 + threadIdx.x) * VEC);
     } else {
-        for (int64_t k = threadIdx.x; k < left; k += 256) {
-            const double g = (double)load_one<DT>(src, at + k);
+        const int whole = (int)(left / VEC), rest = (int)(left % VEC);
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int v = k * 256 + threadIdx.x;
+            p[k] = {};
+            if (v < whole) p[k] = load_words<DT, VEC>(src, at + (int64_t)v * VEC);
+        }
+        acc = (int)threadIdx.x < rest ? (double)load_one<DT>(src, at + (int64_t)whole * VEC + threadIdx.x) : 0.0;
+        acc *= acc;
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const double g = (double)p[k].get(j);
             acc = fma(g, g, acc);
         }
-    }
     return acc;
 }
 
@@ -83,19 +90,24 @@ __global__ void __launch_bounds__(1024) k_norm_final(const double *partial, int 
 
 template <int SD, int DD, int U> __device__ __forceinline__ void scale_chunk(const void *src, void *dst, int64_t at, int64_t left, float scale) {
     constexpr int VEC = Elem<SD>::VEC;
-    if (left >= (int64_t)U * 256 * VEC) {
-        Pack<typename Elem<SD>::T, VEC> p[U];
+    const int whole = (int)(min(left, (int64_t)U * 256 * VEC) / VEC);
+    const int64_t end = at + (int64_t)whole * VEC + threadIdx.x;
+    if (left < (int64_t)U * 256 * VEC && (int)threadIdx.x < (int)(left % VEC)) store_one<DD>(dst, end, load_one<SD>(src, end) * scale);
+    Words<SD, VEC> p[U];
 #pragma unroll
-        for (int k = 0; k < U; ++k) p[k] = load_pack<SD, VEC>(src, at + ((int64_t)k * 256 + threadIdx.x) * VEC);
+    for (int k = 0; k < U; ++k) {
+        const int v = k * 256 + threadIdx.x;
+        if (v < whole) p[k] = load_words<SD, VEC>(src, at + (int64_t)v * VEC);
+    }
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
-            Pack<typename Elem<DD>::T, VEC> q;
+    for (int k = 0; k < U; ++k) {
+        const int v = k * 256 + threadIdx.x;
+        if (v < whole) {
+            Words<DD, VEC> q;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) q.v[j] = Elem<DD>::down(Elem<SD>::up(p[k].v[j]) * scale);
-            store_pack<DD, VEC>(dst, at + ((int64_t)k * 256 + threadIdx.x) * VEC, q);
+            for (int j = 0; j < VEC / 2; ++j) q.set_pair(j, p[k].get(2 * j) * scale, p[k].get(2 * j + 1) * scale);
+            store_words<DD, VEC>(dst, at + (int64_t)v * VEC, q);
         }
-    } else {
-        for (int64_t k = threadIdx.x; k < left; k += 256) store_one<DD>(dst, at + k, load_one<SD>(src, at + k) * scale);
     }
 }
 

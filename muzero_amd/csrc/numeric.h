@@ -32,22 +32,54 @@ template <> struct Elem<MZ_F16> {
     static __device__ __forceinline__ uint16_t down(float f) { const _Float16 h = (_Float16)f; uint16_t v; __builtin_memcpy(&v, &h, 2); return v; }
 };
 
-// N elements of 16 or 32 bits that lie together.  Global loads and stores of this target may start at any element, so rows and
-// views that begin at an odd element take the same 16-byte accesses as aligned ones.
-template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) Pack { T v[N]; };
+// N elements as the 32-bit words that hold them (16-bit ones stay in pairs, half the registers of one word each)
+template <int DT, int N> struct Words {
+    static constexpr int SIZE = sizeof(typename Elem<DT>::T), COUNT = N * SIZE / 4;
+    uint32_t w[COUNT];
+    __device__ __forceinline__ float get(int j) const {
+        if constexpr (DT == MZ_F32) return __uint_as_float(w[j]);
+        else if constexpr (DT == MZ_BF16) return __uint_as_float(j & 1 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
+        else return Elem<DT>::up((uint16_t)(j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xFFFFu));
+    }
+    __device__ __forceinline__ void set(int j, typename Elem<DT>::T v) {
+        if constexpr (DT == MZ_F32) w[j] = v;
+        else w[j / 2] = j & 1 ? (w[j / 2] & 0xFFFFu) | (uint32_t)v << 16 : (w[j / 2] & 0xFFFF0000u) | v;
+    }
+    // elements 2 j and 2 j + 1, each rounded once
+    __device__ __forceinline__ void set_pair(int j, float a, float b) {
+        if constexpr (DT == MZ_F32) {
+            w[2 * j] = __float_as_uint(a);
+            w[2 * j + 1] = __float_as_uint(b);
+        } else {
+            typedef float F2 __attribute__((ext_vector_type(2)));
+            typedef __bf16 B2 __attribute__((ext_vector_type(2)));
+            typedef _Float16 H2 __attribute__((ext_vector_type(2)));
+            const F2 f = {a, b};
+            if constexpr (DT == MZ_BF16) {
+                const B2 h = __builtin_convertvector(f, B2);
+                __builtin_memcpy(&w[j], &h, 4);
+            } else {
+                const H2 h = __builtin_convertvector(f, H2);
+                __builtin_memcpy(&w[j], &h, 4);
+            }
+        }
+    }
+};
 
-template <int DT, int N> __device__ __forceinline__ Pack<typename Elem<DT>::T, N> load_pack(const void *base, int64_t at) {
-    typedef Pack<typename Elem<DT>::T, N> P;
-    const MZ_GLOBAL P *p = (const MZ_GLOBAL P *)((const MZ_GLOBAL typename Elem<DT>::T *)base + at);
-    P r;
-    __builtin_memcpy(&r, p, sizeof(P));
+// Global loads and stores of this target may start at any element, so rows and views that begin at an odd one take the same 16-byte
+// accesses as aligned ones.
+template <int DT, int N> __device__ __forceinline__ Words<DT, N> load_words(const void *base, int64_t at) {
+    Words<DT, N> r;
+    __builtin_memcpy(r.w, (const MZ_GLOBAL typename Elem<DT>::T *)base + at, sizeof(r.w));
     return r;
 }
-template <int DT, int N> __device__ __forceinline__ void store_pack(void *base, int64_t at, const Pack<typename Elem<DT>::T, N> &r) {
-    typedef Pack<typename Elem<DT>::T, N> P;
-    MZ_GLOBAL P *p = (MZ_GLOBAL P *)((MZ_GLOBAL typename Elem<DT>::T *)base + at);
-    __builtin_memcpy(p, &r, sizeof(P));
+template <int DT, int N> __device__ __forceinline__ void store_words(void *base, int64_t at, const Words<DT, N> &r) {
+    __builtin_memcpy((MZ_GLOBAL typename Elem<DT>::T *)base + at, r.w, sizeof(r.w));
 }
+// eight truth values of a byte each, from any address
+struct __attribute__((packed, aligned(1))) Flags { uint64_t v; };
+__device__ __forceinline__ uint64_t load_flags(const uint8_t *base, int64_t at) { return ((const MZ_GLOBAL Flags *)((const MZ_GLOBAL uint8_t *)base + at))->v; }
+
 template <int DT> __device__ __forceinline__ float load_one(const void *base, int64_t at) {
     return Elem<DT>::up(((const MZ_GLOBAL typename Elem<DT>::T *)base)[at]);
 }

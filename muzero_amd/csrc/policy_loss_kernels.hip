@@ -128,58 +128,69 @@ template <int XD, int TD, int E> __global__ void __launch_bounds__(256) k_loss_w
     }
 }
 
+// e^d for d <= 0.  16-bit logits: 2^(d log2 e) on the hardware's exponential, |d| 2^-24 relative, far below a step of theirs; f32 ones: exact to the
+// last places.
+template <int XD> __device__ __forceinline__ float exp_of(float d) { return XD == MZ_F32 ? expf(d) : __builtin_amdgcn_exp2f(d * 1.44269504f); }
+
 // ---- a run of VEC actions in registers ---------------------------------------------------------------------------------------
 template <int XD, int TD> struct Run {
     static constexpr int VEC = Elem<XD>::VEC;
-    Pack<typename Elem<XD>::T, VEC> x;
-    Pack<typename Elem<TD>::T, VEC> t;
+    Words<XD, VEC> x;
+    Words<TD, VEC> t;
     // actions at..at+VEC-1 of a row; what lies behind its end or is not legal becomes x = -inf, t = 0
     __device__ __forceinline__ void load(const LossArgs &A, int64_t xo, int64_t to, int64_t ao, int at) {
         if (at + VEC <= A.v) {
-            x = load_pack<XD, VEC>(A.x, xo + at);
-            t = load_pack<TD, VEC>(A.t, to + at);
+            x = load_words<XD, VEC>(A.x, xo + at);
+            t = load_words<TD, VEC>(A.t, to + at);
             if (A.allowed) {
-                Pack<uint8_t, VEC> ok;
-                __builtin_memcpy(&ok, A.allowed + ao + at, VEC);
+                uint32_t ok[VEC / 4];
+                __builtin_memcpy(ok, (const MZ_GLOBAL uint8_t *)A.allowed + ao + at, VEC);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j)
-                    if (!ok.v[j]) clear(j);
+                    if (!((ok[j / 4] >> (j & 3) * 8) & 0xFF)) clear(j);
             }
         } else {
+            x = {};
+            t = {};
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 clear(j);
                 if (at + j < A.v && (!A.allowed || A.allowed[ao + at + j])) {
-                    x.v[j] = ((const MZ_GLOBAL typename Elem<XD>::T *)A.x)[xo + at + j];
-                    t.v[j] = ((const MZ_GLOBAL typename Elem<TD>::T *)A.t)[to + at + j];
+                    x.set(j, ((const MZ_GLOBAL typename Elem<XD>::T *)A.x)[xo + at + j]);
+                    t.set(j, ((const MZ_GLOBAL typename Elem<TD>::T *)A.t)[to + at + j]);
                 }
             }
         }
     }
     __device__ __forceinline__ void clear(int j) {
-        x.v[j] = XD == MZ_F32 ? 0xFF800000u : XD == MZ_BF16 ? 0xFF80u : 0xFC00u;
-        t.v[j] = 0;
+        x.set(j, XD == MZ_F32 ? 0xFF800000u : XD == MZ_BF16 ? 0xFF80u : 0xFC00u);
+        t.set(j, 0);
     }
-    __device__ __forceinline__ float xf(int j) const { return Elem<XD>::up(x.v[j]); }
-    __device__ __forceinline__ float tf(int j) const { return Elem<TD>::up(t.v[j]); }
+    __device__ __forceinline__ float xf(int j) const { return x.get(j); }
+    __device__ __forceinline__ float tf(int j) const { return t.get(j); }
     __device__ __forceinline__ void add(Stat &s, float shift) const {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
             const float d = xf(j) - shift, tv = tf(j);
-            s.z += expf(d);
+            s.z += exp_of<XD>(d);
             s.t += tv;
             if (tv != 0.0f) s.a = fmaf(tv, d, s.a);
         }
     }
     __device__ __forceinline__ void store_grad(const LossArgs &A, int64_t go, int at, bool zero, float shift, float tz, float scale) const {
-        Pack<typename Elem<XD>::T, VEC> g;
+        Words<XD, VEC> g;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) g.v[j] = Elem<XD>::down(zero ? 0.0f : (expf(xf(j) - shift) * tz - tf(j)) * scale);
-        if (at + VEC <= A.v) store_pack<XD, VEC>(A.grad, go + at, g);
+        for (int j = 0; j < VEC / 2; ++j) {
+            float f[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) f[i] = zero ? 0.0f : fmaf(exp_of<XD>(xf(2 * j + i) - shift), tz, -tf(2 * j + i)) * scale;
+            g.set_pair(j, f[0], f[1]);
+        }
+        if (at + VEC <= A.v) store_words<XD, VEC>(A.grad, go + at, g);
         else {
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
-                if (at + j < A.v) ((MZ_GLOBAL typename Elem<XD>::T *)A.grad)[go + at + j] = g.v[j];
+                if (at + j < A.v) store_one<XD>(A.grad, go + at + j, g.get(j));
         }
     }
 };

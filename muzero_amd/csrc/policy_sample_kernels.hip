@@ -244,14 +244,13 @@ constexpr int BINS = 1024;
 // eight actions of a row; what lies behind its end or is not legal is -inf
 template <int XD> __device__ __forceinline__ void load_eight(const SampleArgs &A, int64_t xo, int64_t ao, int at, float *x) {
     if (at + 8 <= A.v) {
-        const Pack<typename Elem<XD>::T, 8> p = load_pack<XD, 8>(A.x, xo + at);
+        const Words<XD, 8> p = load_words<XD, 8>(A.x, xo + at);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = Elem<XD>::up(p.v[j]);
+        for (int j = 0; j < 8; ++j) x[j] = p.get(j);
         if (A.allowed) {
-            Pack<uint8_t, 8> ok;
-            __builtin_memcpy(&ok, A.allowed + ao + at, 8);
+            const uint64_t ok = load_flags(A.allowed, ao + at);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = ok.v[j] ? x[j] : -INFINITY;
+            for (int j = 0; j < 8; ++j) x[j] = (ok >> j * 8) & 0xFF ? x[j] : -INFINITY;
         }
     } else {
 #pragma unroll
