@@ -163,7 +163,7 @@ template <int XD, int TD> struct Run {
         }
     }
     __device__ __forceinline__ void clear(int j) {
-        x.set(j, XD == MZ_F32 ? 0xFF800000u : XD == MZ_BF16 ? 0xFF80u : 0xFC00u);
+        x.set(j, (typename Elem<XD>::T)(XD == MZ_F32 ? 0xFF800000u : XD == MZ_BF16 ? 0xFF80u : 0xFC00u));
         t.set(j, 0);
     }
     __device__ __forceinline__ float xf(int j) const { return x.get(j); }
@@ -342,7 +342,7 @@ template <int XD, int TD> int launch(const LossArgs &A, Stat *part, hipStream_t 
     else if (!few && vecs <= 256 * 2) hipLaunchKernelGGL((k_loss_row<XD, TD, 256, 2>), dim3(rows), dim3(256), 0, s, A);
     else if (!few && vecs <= 256 * 4) hipLaunchKernelGGL((k_loss_row<XD, TD, 256, 4>), dim3(rows), dim3(256), 0, s, A);
     else if (!few && vecs <= 512 * 4) hipLaunchKernelGGL((k_loss_row<XD, TD, 512, 4>), dim3(rows), dim3(512), 0, s, A);
-    else if (!few && vecs <= 1024 * 4) hipLaunchKernelGGL((k_loss_row<XD, TD, 1024, 4>), dim3(rows), dim3(1024), 0, s, A);
+    else if (!few && vecs <= 512 * 8) hipLaunchKernelGGL((k_loss_row<XD, TD, 512, 8>), dim3(rows), dim3(512), 0, s, A);
     else {
         const Plan p = plan_chunks(A.n, A.v, elem_bytes(XD) + elem_bytes(TD));
         for (int64_t r = 0; r < A.n; r += p.slab) {

@@ -10,10 +10,10 @@
 // All masses are held in 64 bits, because a draw next to the border of two actions has to fall on its own side: at 131,072 actions f32 sums would put
 // one draw in a thousand wrong.  Sums run in a fixed order, or over integers (w scaled to 2^s, so that atomics give the same total in any order).
 //
-// Short rows (up to 512 actions): one wave per row, everything in registers, thresholds bit by bit.
-// Long rows, two launches: k_sample_groups reads the logits once, across all CUs, and leaves the maximum of every 128 actions and, where the
-// row's settings need the total, their mass; k_sample_row, a workgroup per row, works from those: it finds a lower bound of what can be
-// kept, reads again only the groups that reach it, and finds the thresholds by histograms over the logits' bits, 1024 bins at a time.
+// Up to 512 actions: one wave per row.  Up to 8192: one workgroup of 4, 8 or 16 waves per row.  Both hold the row in registers, one launch.
+// Longer rows, two launches: k_sample_groups reads the logits once, across all CUs, and leaves the maximum of every 128 actions and, where the
+// row's settings need the total, their mass.  k_sample_row, a workgroup per row, works from those: bounds on what can be kept leave few groups, it
+// reads only these again, takes the actions above the bound into registers (up to 4096 or 8192) and goes on as for a shorter row.
 #include <math.h>
 #include <algorithm>
 #include "numeric.h"
@@ -67,57 +67,70 @@ constexpr uint32_t KEY_NONE = 0x007FFFFFu;     // -inf: an action that cannot be
 constexpr uint32_t KEY_LOWEST = 0x00800000u;   // the lowest finite value
 constexpr uint32_t KEY_INF = 0xFF800000u;      // +inf, and above it NaN: no distribution
 
-// 2^t for t <= 0: 2^round(t) times the series of e^y at y = ln 2 (t - round(t)), |y| <= 0.3466; y^13 / 13! < 2e-16
+// 2^t for t <= 0: 2^round(t) times a polynomial at f = t - round(t) in [-1/2, 1/2], 1 + f q(f) with q the interpolation of (2^f - 1) / f at the
+// Chebyshev nodes of degree 9 (relative error 6e-16; 2^0 is 1 exactly)
 __device__ __forceinline__ double exp2_neg(double t) {
     t = fmax(t, -1100.0);
-    const double r = rint(t);
-    const double y = (t - r) * 0.6931471805599453;
-    double q = 1.0 / 479001600.0;
-    q = fma(q, y, 1.0 / 39916800.0);
-    q = fma(q, y, 1.0 / 3628800.0);
-    q = fma(q, y, 1.0 / 362880.0);
-    q = fma(q, y, 1.0 / 40320.0);
-    q = fma(q, y, 1.0 / 5040.0);
-    q = fma(q, y, 1.0 / 720.0);
-    q = fma(q, y, 1.0 / 120.0);
-    q = fma(q, y, 1.0 / 24.0);
-    q = fma(q, y, 1.0 / 6.0);
-    q = fma(q, y, 0.5);
-    q = fma(q, y, 1.0);
-    q = fma(q, y, 1.0);
+    const double r = rint(t), f = t - r;
+    double q = 7.070977866508138e-09;
+    q = fma(q, f, 1.0205905413765595e-07);
+    q = fma(q, f, 1.3215451633221434e-06);
+    q = fma(q, f, 1.5252672924850737e-05);
+    q = fma(q, f, 0.00015403530424776529);
+    q = fma(q, f, 0.0013333558200794592);
+    q = fma(q, f, 0.009618129107618665);
+    q = fma(q, f, 0.05550410866465167);
+    q = fma(q, f, 0.24022650695910075);
+    q = fma(q, f, 0.6931471805599462);
+    q = fma(q, f, 1.0);
     return ldexp(q, (int)r);
 }
 __device__ __forceinline__ double mass_of(float x, double m, double c) { return exp2_neg(((double)x - m) * c); }
 
-__device__ __forceinline__ double wave_scan(double v, int lane) {   // inclusive
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const double o = __shfl_up(v, d, 64);
-        if (lane >= d) v += o;
-    }
+// ---- reductions and scans over a wave in registers: rows of 16 lanes by shifts, then across the rows (lanes that get nothing add 0) ----------
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false); }
+template <int CTRL, int ROWS> __device__ __forceinline__ double dpp(double v) {
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    return __longlong_as_double((long long)((uint64_t)dpp<CTRL, ROWS>((uint32_t)(b >> 32)) << 32 | dpp<CTRL, ROWS>((uint32_t)b)));
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ uint64_t dpp(uint64_t v) {
+    return (uint64_t)dpp<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | dpp<CTRL, ROWS>((uint32_t)v);
+}
+template <typename T> __device__ __forceinline__ T scan(T v) {   // inclusive
+    v += dpp<0x111, 0xF>(v);
+    v += dpp<0x112, 0xF>(v);
+    v += dpp<0x114, 0xF>(v);
+    v += dpp<0x118, 0xF>(v);
+    v += dpp<0x142, 0xA>(v);
+    v += dpp<0x143, 0xC>(v);
     return v;
 }
-__device__ __forceinline__ int wave_scan_int(int v, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(v, d, 64);
-        if (lane >= d) v += o;
-    }
-    return v;
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) { return (uint64_t)lane_of((uint32_t)(v >> 32), lane) << 32 | lane_of((uint32_t)v, lane); }
+__device__ __forceinline__ double lane_of(double v, int lane) { return __longlong_as_double((long long)lane_of((uint64_t)__double_as_longlong(v), lane)); }
+template <typename T> __device__ __forceinline__ T total(T v) { return lane_of(scan(v), 63); }
+// the largest over 16 lanes in their last one, and over the wave in every lane
+__device__ __forceinline__ uint32_t max16(uint32_t v) {
+    v = max(v, dpp<0x111, 0xF>(v));
+    v = max(v, dpp<0x112, 0xF>(v));
+    v = max(v, dpp<0x114, 0xF>(v));
+    return max(v, dpp<0x118, 0xF>(v));
 }
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d, 64));
-    return v;
+    v = max16(v);
+    v = max(v, dpp<0x142, 0xA>(v));
+    return lane_of(max(v, dpp<0x143, 0xC>(v)), 63);
 }
-__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v += (uint64_t)__shfl_xor((long long)v, d, 64);
-    return v;
+__device__ __forceinline__ uint32_t lane_last16(uint32_t v) { return (uint32_t)__builtin_amdgcn_ds_swizzle((int)v, 0x1F0); }   // lane 15 of each 16
+__device__ __forceinline__ double sum16(double v) {   // in the last of 16 lanes
+    v += dpp<0x111, 0xF>(v);
+    v += dpp<0x112, 0xF>(v);
+    v += dpp<0x114, 0xF>(v);
+    return v + dpp<0x118, 0xF>(v);
 }
 __device__ __forceinline__ uint64_t lanes_below(int lane) { return lane ? ~0ull >> (64 - lane) : 0ull; }
 
-// ---- short rows: one wave each, action j = 64 k + lane --------------------------------------------------------------------------------
+// ---- up to 512 actions: one wave per row, action j = 64 k + lane ---------------------------------------------------------------------
 template <int XD, int E> __global__ void __launch_bounds__(256) k_sample_wave(SampleArgs A) {
     const int lane = threadIdx.x & 63;
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -176,18 +189,22 @@ template <int XD, int E> __global__ void __launch_bounds__(256) k_sample_wave(Sa
         }
         if (s.p_on) {   // the lowest tau above which less than p of the mass lies
             const double w_tau = tau > KEY_NONE ? mass_of(value_of(tau), m, s.c) : 0.0;
-            double total = 0.0;
+            double all = 0.0;
+            uint32_t lo = 0xFFFFFFFFu, hi = top;
 #pragma unroll
-            for (int k = 0; k < E; ++k) total += key[k] > tau ? w[k] : 0.0;
-            total = wave_sum(total) + (tau > KEY_NONE ? ties * w_tau : 0.0);
-            const double limit = s.top_p * total;
-            uint32_t lo = tau > KEY_NONE ? tau : KEY_LOWEST, hi = top;   // the answer lies in [lo, hi]: nothing is above the largest key
+            for (int k = 0; k < E; ++k) {
+                all += key[k] > tau ? w[k] : 0.0;
+                if (key[k] > KEY_NONE && key[k] >= tau) lo = min(lo, key[k]);
+            }
+            all = total(all) + (tau > KEY_NONE ? ties * w_tau : 0.0);
+            const double limit = s.top_p * all;
+            lo = ~wave_max_u32(~lo);             // the answer lies in [lo, hi]: the least key that can be kept, and the largest, above which nothing is
             while (lo < hi) {
                 const uint32_t mid = lo + (hi - lo) / 2;
                 double above = 0.0;
 #pragma unroll
                 for (int k = 0; k < E; ++k) above += key[k] > mid ? w[k] : 0.0;
-                if (wave_sum(above) < limit) hi = mid;
+                if (total(above) < limit) hi = mid;
                 else lo = mid + 1;
             }
             double above = 0.0;
@@ -197,7 +214,7 @@ template <int XD, int E> __global__ void __launch_bounds__(256) k_sample_wave(Sa
                 above += key[k] > lo ? w[k] : 0.0;
                 on += __popcll(__ballot(key[k] == lo));
             }
-            above = wave_sum(above);
+            above = total(above);
             const double wl = mass_of(value_of(lo), m, s.c);
             int r = 0;
             while (r < on && above + r * wl < limit) ++r;
@@ -221,8 +238,8 @@ template <int XD, int E> __global__ void __launch_bounds__(256) k_sample_wave(Sa
         keep[k] = __ballot(kept);
         part[k] = 0.0;
         if (keep[k]) {
-            part[k] = base + wave_scan(kept ? w[k] : 0.0, lane);
-            base = __shfl(part[k], 63, 64);
+            part[k] = base + scan(kept ? w[k] : 0.0);
+            base = lane_of(part[k], 63);
         }
     }
     const double target = A.u[row] * base;
@@ -235,11 +252,6 @@ template <int XD, int E> __global__ void __launch_bounds__(256) k_sample_wave(Sa
     }
     if (lane == 0) A.action[row] = pick < 0 ? last : pick;
 }
-
-// ---- long rows ------------------------------------------------------------------------------------------------------------------------
-constexpr int GROUP = 128;          // actions whose maximum and mass are kept together: 16 lanes of 8
-constexpr int MAX_V = 1 << 19;      // 4096 groups: 48 KB of LDS for a row
-constexpr int BINS = 1024;
 
 // eight actions of a row; what lies behind its end or is not legal is -inf
 template <int XD> __device__ __forceinline__ void load_eight(const SampleArgs &A, int64_t xo, int64_t ao, int at, float *x) {
@@ -258,6 +270,304 @@ template <int XD> __device__ __forceinline__ void load_eight(const SampleArgs &A
     }
 }
 
+// ---- what a workgroup of W waves does together -----------------------------------------------------------------------------------------
+template <int W> struct Shared {
+    static constexpr int THREADS = 64 * W, BINS = 4 * THREADS, FEW = 64;
+    unsigned long long hist[BINS];
+    unsigned long long few_amount[FEW];
+    uint32_t few_key[FEW];
+    unsigned long long wave_u64[W];
+    double wave_f64[W];
+    uint32_t wave_u32[W];
+    unsigned long long above;
+    double base;
+    int bin, few, pick;
+};
+
+template <int W, typename T> __device__ __forceinline__ T block_total(T v, T *of_wave) {   // of_wave may be used again after the call
+    v = total(v);
+    if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = v;
+    __syncthreads();
+    T t = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) t += of_wave[i];
+    __syncthreads();
+    return t;
+}
+template <int W> __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t *of_wave) {
+    v = wave_max_u32(v);
+    if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = v;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < W; ++i) v = max(v, of_wave[i]);
+    __syncthreads();
+    return v;
+}
+
+// The bin of the histogram that takes the amounts from below `limit` to it, counted from bin 0; -1: their total stays below.  `above`: what lies
+// in the bins before it, on entry and on return together with what was there.
+template <int W> __device__ __forceinline__ int crossing_bin(Shared<W> &S, uint64_t limit, uint64_t *above) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint64_t h[4], own = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) own += h[i] = S.hist[threadIdx.x * 4 + i];
+    const uint64_t sum = scan(own);
+    if (lane == 63) S.wave_u64[wave] = sum;
+    __syncthreads();
+    uint64_t before = *above + sum - own;
+    for (int i = 0; i < wave; ++i) before += S.wave_u64[i];
+    if (before < limit && before + own >= limit) {   // one thread at most
+        int i = 0;
+        while (before + h[0] < limit) {
+            before += h[0];
+            h[0] = h[1];
+            h[1] = h[2];
+            h[2] = h[3];
+            ++i;
+        }
+        S.bin = threadIdx.x * 4 + i;
+        S.above = before;
+    }
+    __syncthreads();
+    if (S.bin >= 0) *above = S.above;
+    return S.bin;
+}
+
+// The lowest tau in [lo, hi] with (amount above tau) < limit, where `each` hands (key, value, function of the amount) of everything in the row to
+// its argument; *above = that amount.  False: all of it together stays below the limit.  Amounts are integers, so the order of the atomics does
+// not matter.  `lo` may be lowered by nothing; `ends` = bits of a key that its type leaves empty.
+// The first histogram has bins of equal width in the value, which few logits share; the up to 64 of the bin that reaches the limit are ranked in
+// registers.  More (equal logits): histograms over the keys' bits, each narrowing to one bin of the one before.
+template <int W, class EACH> __device__ __forceinline__ bool find_threshold(EACH each, uint32_t lo, uint32_t hi, uint64_t limit, int ends, Shared<W> &S, uint32_t *tau, uint64_t *above_out) {
+    constexpr int BINS = Shared<W>::BINS, BITS = W == 4 ? 10 : W == 8 ? 11 : 12, FEW = Shared<W>::FEW;
+    static_assert(1 << BITS == BINS, "a bin for each key of that many bits");
+    const int lane = threadIdx.x & 63;
+    auto clear = [&] {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) S.hist[threadIdx.x * 4 + i] = 0;
+        if (threadIdx.x == 0) {
+            S.bin = -1;
+            S.few = 0;
+        }
+        __syncthreads();
+    };
+    uint64_t above = 0;
+    const float xh = value_of(hi), width = xh - value_of(lo), scale = BINS / width;
+    if (((hi - lo) >> ends) >= BINS && scale > 0.0f && scale < 1e30f) {
+        auto bin_of = [&](float x) { return min(BINS - 1, (int)((xh - x) * scale)); };
+        clear();
+        each([&](uint32_t key, float x, auto amount) {
+            if (key >= lo && key <= hi) atomicAdd(&S.hist[bin_of(x)], (unsigned long long)amount());
+        });
+        __syncthreads();
+        const int bin = crossing_bin(S, limit, &above);
+        if (bin < 0) return false;
+        each([&](uint32_t key, float x, auto amount) {
+            if (key >= lo && key <= hi && bin_of(x) == bin) {
+                const int i = atomicAdd(&S.few, 1);
+                if (i < FEW) {
+                    S.few_key[i] = key;
+                    S.few_amount[i] = (unsigned long long)amount();
+                }
+            }
+        });
+        __syncthreads();
+        const int few = S.few;
+        if (few <= FEW) {
+            const uint32_t key = lane < few ? S.few_key[lane] : 0;
+            const uint64_t amount = lane < few ? (uint64_t)S.few_amount[lane] : 0;
+            uint64_t over = above;
+            for (int i = 0; i < few; ++i) {
+                const uint32_t k = lane_of(key, i);
+                const uint64_t a = lane_of(amount, i);
+                if (k > key) over += a;
+            }
+            const uint32_t best = lane < few && over < limit ? key : 0xFFFFFFFFu;
+            *tau = ~wave_max_u32(~best);
+            *above_out = lane_of(over, __ffsll((unsigned long long)__ballot(best == *tau)) - 1);
+            return true;
+        }
+        above = 0;
+    }
+    for (;;) {
+        const int shift = max(0, 32 - __clz((int)(hi - lo)) - BITS);   // (hi - lo) >> shift < BINS
+        clear();
+        each([&](uint32_t key, float, auto amount) {
+            if (key >= lo && key <= hi) atomicAdd(&S.hist[(hi - key) >> shift], (unsigned long long)amount());
+        });
+        __syncthreads();
+        const int bin = crossing_bin(S, limit, &above);
+        if (bin < 0) return false;
+        hi -= (uint32_t)bin << shift;
+        if (shift <= ends) {      // one key: the one whose low bits are what its type leaves there, 0 above zero and 1 below
+            const uint32_t low = (1u << ends) - 1;
+            uint32_t t = hi & 0x80000000u ? hi & ~low : hi | low;
+            if (t > hi) t -= low + 1;
+            *tau = t;
+            *above_out = above;
+            return true;
+        }
+        lo = hi - lo < (1u << shift) ? lo : hi - (1u << shift) + 1;
+    }
+}
+template <int XD> constexpr int key_ends() { return XD == MZ_F32 ? 0 : XD == MZ_BF16 ? 16 : 13; }
+
+// masses as integers: at most 2^50 each, their sum over v actions below 2^63
+__device__ __forceinline__ double int_scale(int v) { return ldexp(1.0, min(50, 62 - (32 - __clz(v)))); }
+__device__ __forceinline__ uint64_t int_mass(double w, double scale) {   // the mantissa of w scale + 2^52 holds it, rounded
+    return (uint64_t)__double_as_longlong(fma(w, scale, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
+}
+
+// The answer for what the workgroup's threads hold in registers, thread by thread in the actions' order, N in each: the place of the picked one
+// (thread N + j), in every thread.  best: the largest key.  low: nothing below it is kept.  all: the mass that top-p shares out, if it is known (> 0).
+template <int XD, int W, int N> __device__ __forceinline__ int pick(const float *x, const Setting &s, double u, int v, uint32_t best, uint32_t low, double all, Shared<W> &S) {
+    constexpr int ENDS = key_ends<XD>();
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const double m = (double)value_of(best);
+    uint32_t tau = KEY_NONE, ties = 0;           // the kept set: keys above tau, and the first `ties` on it
+    double w[N];
+    if (s.greedy) {
+        tau = best - 1;
+#pragma unroll
+        for (int j = 0; j < N; ++j) w[j] = 1.0;
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) w[j] = mass_of(x[j], m, s.c);
+        uint64_t above;
+        if (low == KEY_LOWEST && (s.k || s.p_on)) {   // no bound yet: the least value that is there
+            uint32_t least = 0xFFFFFFFFu;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const uint32_t key = key_of(x[j]);
+                if (key > KEY_NONE) least = min(least, key);
+            }
+            low = ~block_max<W>(~least, S.wave_u32);
+        }
+        if (s.k) {
+            auto each = [&](auto take) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) take(key_of(x[j]), x[j], [] { return 1ull; });
+            };
+            uint32_t t;
+            if (find_threshold(each, low, best, (uint64_t)s.k, ENDS, S, &t, &above)) {
+                tau = t;
+                ties = (uint32_t)(s.k - above);
+            }
+        }
+        if (s.p_on) {
+            const uint32_t lowest = tau > KEY_NONE ? tau : low;
+            const double scale = int_scale(v);
+            double limit;
+            if (all > 0.0) limit = s.top_p * all * scale;
+            else {
+                uint64_t sum = 0;
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const uint32_t key = key_of(x[j]);
+                    if (key > tau && key >= lowest) sum += int_mass(w[j], scale);
+                }
+                sum = block_total<W>(sum, (uint64_t *)S.wave_u64);
+                if (tau > KEY_NONE) sum += ties * int_mass(mass_of(value_of(tau), m, s.c), scale);
+                limit = s.top_p * (double)sum;
+            }
+            const uint64_t amount = (uint64_t)fmax(1.0, ceil(limit));
+            auto each = [&](auto take) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) take(key_of(x[j]), x[j], [&] { return int_mass(w[j], scale); });
+            };
+            uint32_t t;
+            if (find_threshold(each, lowest, best, amount, ENDS, S, &t, &above)) {
+                const uint64_t one = max((uint64_t)1, int_mass(mass_of(value_of(t), m, s.c), scale));
+                const uint32_t r = (uint32_t)min((amount - above + one - 1) / one, (uint64_t)v);
+                if (t > tau) {
+                    tau = t;
+                    ties = r;
+                } else ties = min(ties, r);
+            }
+        }
+    }
+    // cumulated in the actions' order
+    uint32_t on = 0;
+    if (tau > KEY_NONE)
+#pragma unroll
+        for (int j = 0; j < N; ++j) on += key_of(x[j]) == tau;
+    const uint32_t on_upto = scan(on);
+    __syncthreads();
+    if (lane == 63) S.wave_u32[wave] = on_upto;
+    if (threadIdx.x == 0) S.pick = 0x7FFFFFFF;
+    __syncthreads();
+    uint32_t rank = on_upto - on;
+    for (int i = 0; i < wave; ++i) rank += S.wave_u32[i];
+    double own = 0.0;
+    uint32_t keep = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint32_t key = key_of(x[j]);
+        bool kept = key > tau;
+        if (key == tau && on) kept = rank++ < ties;
+        if (!s.greedy && s.m_on) kept = kept && (w[j] >= s.min_p || key == best);
+        if (kept) {
+            keep |= 1u << j;
+            own += w[j];
+        }
+    }
+    const double sum = scan(own);
+    if (lane == 63) S.wave_f64[wave] = sum;
+    __syncthreads();
+    double cum = sum - own, everything = 0.0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        cum += i < wave ? S.wave_f64[i] : 0.0;
+        everything += S.wave_f64[i];
+    }
+    const double target = s.greedy ? -1.0 : u * everything;
+    int mine = -1, last = -1;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+        if (keep >> j & 1) {
+            cum += w[j];
+            last = j;
+            if (mine < 0 && cum > target) mine = j;
+        }
+    if (mine >= 0) atomicMin(&S.pick, (int)threadIdx.x * N + mine);
+    __syncthreads();
+    int at = S.pick;
+    if (at == 0x7FFFFFFF) {                      // rounding, or u >= 1: the last that is kept
+        __syncthreads();
+        if (threadIdx.x == 0) S.pick = -1;
+        __syncthreads();
+        if (last >= 0) atomicMax(&S.pick, (int)threadIdx.x * N + last);
+        __syncthreads();
+        at = S.pick;
+    }
+    return at;
+}
+
+// ---- up to 512 W actions: a workgroup of W waves per row, eight neighbouring actions in a thread -----------------------------------------
+template <int XD, int W> __global__ void __launch_bounds__(64 * W) k_sample_block(SampleArgs A) {
+    __shared__ Shared<W> S;
+    const int64_t row = blockIdx.x;
+    const Setting s = setting_of(A, row);
+    float x[8];
+    load_eight<XD>(A, row * A.x_stride, row * A.allowed_stride, threadIdx.x * 8, x);
+    uint32_t best = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) best = max(best, x[j] != x[j] ? 0xFFFFFFFFu : key_of(x[j]));
+    best = block_max<W>(best, S.wave_u32);
+    if (best <= KEY_NONE || best >= KEY_INF || s.bad) {
+        if (threadIdx.x == 0) A.action[row] = -1;
+        return;
+    }
+    const int at = pick<XD, W, 8>(x, s, A.u[row], A.v, best, KEY_LOWEST, 0.0, S);
+    if (threadIdx.x == 0) A.action[row] = at;
+}
+
+// ---- longer rows ---------------------------------------------------------------------------------------------------------------------
+constexpr int GROUP = 128;          // actions whose maximum and mass are kept together: 16 lanes of 8
+constexpr int MAX_V = 1 << 19;      // 4096 groups
+constexpr int BLOCK_V = 8192;       // the longest row that one workgroup holds in registers from the start
+
 // whether a row's total mass has to come from all of its actions
 __device__ __forceinline__ bool needs_mass(const Setting &s) { return !s.greedy && !s.k && (s.p_on || !s.m_on); }
 
@@ -265,10 +575,9 @@ __device__ __forceinline__ bool needs_mass(const Setting &s) { return !s.greedy 
 template <int XD> __global__ void __launch_bounds__(256) k_sample_groups(SampleArgs A, int groups, double *mass, uint32_t *top) {
     const int64_t row = blockIdx.y;
     const int at = blockIdx.x * 2048 + threadIdx.x * 8, g = at / GROUP;
-    if (g >= groups) return;
     const Setting s = setting_of(A, row);
     float x[8];
-    load_eight<XD>(A, row * A.x_stride, row * A.allowed_stride, at, x);
+    load_eight<XD>(A, row * A.x_stride, row * A.allowed_stride, at, x);   // behind the row's end: nothing is read
     float m = -INFINITY;
     bool nan = false;
 #pragma unroll
@@ -276,10 +585,9 @@ template <int XD> __global__ void __launch_bounds__(256) k_sample_groups(SampleA
         m = fmaxf(m, x[j]);
         nan |= x[j] != x[j];
     }
-    uint32_t key = nan ? 0xFFFFFFFFu : key_of(m);
-#pragma unroll
-    for (int d = 8; d; d >>= 1) key = max(key, (uint32_t)__shfl_xor((int)key, d, 16));
-    if ((threadIdx.x & 15) == 0) top[row * groups + g] = key;
+    const uint32_t key = lane_last16(max16(nan ? 0xFFFFFFFFu : key_of(m)));
+    const bool writes = (threadIdx.x & 15) == 15 && g < groups;
+    if (writes) top[row * groups + g] = key;
     if (!needs_mass(s)) return;
     double w = 0.0;
     if (key > KEY_NONE && key < KEY_INF) {
@@ -287,124 +595,64 @@ template <int XD> __global__ void __launch_bounds__(256) k_sample_groups(SampleA
 #pragma unroll
         for (int j = 0; j < 8; ++j) w += mass_of(x[j], md, s.c);
     }
-#pragma unroll
-    for (int d = 8; d; d >>= 1) w += __shfl_xor(w, d, 16);
-    if ((threadIdx.x & 15) == 0) mass[row * groups + g] = w;
+    w = sum16(w);
+    if (writes) mass[row * groups + g] = w;
 }
 
-constexpr int ROW_THREADS = 1024, ROW_WAVES = ROW_THREADS / 64;
-
-struct RowShared {
-    unsigned long long hist[BINS];
-    unsigned long long wave_u64[ROW_WAVES];
-    double wave_f64[ROW_WAVES];
-    uint32_t wave_u32[ROW_WAVES];
-    unsigned long long above;
-    double base;
-    int bin, group;
+// LDS of a row: its groups, then the actions that its bounds leave, SEG to each wave
+template <int W, int N> struct RowShared {
+    static constexpr int SEG = 64 * N;
+    Shared<W> S;
+    float x[W * SEG];
+    int32_t index[W * SEG];
+    int overflow;
 };
 
-__device__ __forceinline__ uint64_t block_sum_u64(uint64_t v, RowShared &S) {
-    v = wave_sum_u64(v);
-    if ((threadIdx.x & 63) == 0) S.wave_u64[threadIdx.x >> 6] = v;
-    __syncthreads();
-    uint64_t t = 0;
-#pragma unroll
-    for (int i = 0; i < ROW_WAVES; ++i) t += S.wave_u64[i];
-    __syncthreads();
-    return t;
-}
-
-// The lowest tau in [lo, hi] with (amount above tau) < limit, where `each` hands every (key, function of its amount) of the row to its argument; `above` = that
-// amount.  Histograms over [lo, hi], the bin that reaches the limit becomes the next range, down to a single key.  Amounts are integers, so the order of
-// the atomics does not matter.  False: all of them together stay below the limit.
-template <class EACH> __device__ bool find_threshold(EACH each, uint32_t lo, uint32_t hi, uint64_t limit, RowShared &S, uint32_t *tau, uint64_t *above_out) {
-    uint64_t above = 0;
-    for (;;) {
-        const uint32_t width = hi - lo;
-        const int shift = max(0, 32 - __clz((int)width) - 10);    // width >> shift < 1024
-        S.hist[threadIdx.x] = 0;
-        if (threadIdx.x == 0) S.bin = -1;
-        __syncthreads();
-        each([&](uint32_t key, auto amount) {
-            if (key >= lo && key <= hi) atomicAdd(&S.hist[(hi - key) >> shift], (unsigned long long)amount());
-        });
-        __syncthreads();
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        const uint64_t own = S.hist[threadIdx.x];
-        uint64_t sum = own;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint64_t o = (uint64_t)__shfl_up((long long)sum, d, 64);
-            if (lane >= d) sum += o;
-        }
-        if (lane == 63) S.wave_u64[wave] = sum;
-        __syncthreads();
-        uint64_t before = above;
-        for (int i = 0; i < wave; ++i) before += S.wave_u64[i];
-        if (before + sum - own < limit && before + sum >= limit) {    // one thread at most
-            S.bin = threadIdx.x;
-            S.above = before + sum - own;
-        }
-        __syncthreads();
-        const int bin = S.bin;
-        above = S.above;
-        __syncthreads();
-        if (bin < 0) return false;
-        hi -= (uint32_t)bin << shift;
-        if (shift == 0) {
-            *tau = hi;
-            *above_out = above;
-            return true;
-        }
-        lo = hi - lo < (1u << shift) ? lo : hi - (1u << shift) + 1;
-    }
-}
-
-template <int XD> __global__ void __launch_bounds__(ROW_THREADS) k_sample_row(SampleArgs A, int groups, const double *mass_in, const uint32_t *top_in) {
+template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_sample_row(SampleArgs A, int groups, const double *mass_in, const uint32_t *top_in) {
+    constexpr int THREADS = 64 * W, SEG = RowShared<W, N>::SEG, ENDS = key_ends<XD>();
+    __shared__ RowShared<W, N> R;
     extern __shared__ double dyn[];
-    __shared__ RowShared S;
+    Shared<W> &S = R.S;
     double *mass = dyn;                          // of a group: all of it, later what is kept of it
     uint32_t *top = (uint32_t *)(dyn + groups);  // its largest key, later how many actions on the threshold come before it
     const int64_t row = blockIdx.x;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Setting s = setting_of(A, row);
     const int64_t xo = row * A.x_stride, ao = row * A.allowed_stride;
-    const bool massed = needs_mass(s);
+    const bool massed = needs_mass(s), filtered = s.k || s.p_on || s.m_on;
 
     uint32_t best = 0;
-    for (int g = threadIdx.x; g < groups; g += ROW_THREADS) {
+    for (int g = threadIdx.x; g < groups; g += THREADS) {
         top[g] = top_in[row * groups + g];
-        mass[g] = massed ? mass_in[row * groups + g] : 0.0;
+        if (massed) mass[g] = mass_in[row * groups + g];
         best = max(best, top[g]);
     }
-    best = wave_max_u32(best);
-    if (lane == 0) S.wave_u32[wave] = best;
-    if (threadIdx.x == 0) S.group = 0x7FFFFFFF;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < ROW_WAVES; ++i) best = max(best, S.wave_u32[i]);
+    if (threadIdx.x == 0) {
+        S.pick = 0x7FFFFFFF;
+        R.overflow = 0;
+    }
+    best = block_max<W>(best, S.wave_u32);
     if (best <= KEY_NONE || best >= KEY_INF || s.bad) {
         if (threadIdx.x == 0) A.action[row] = -1;
         return;
     }
-    const double m = (double)value_of(best);
+    const double m = (double)value_of(best), u = A.u[row];
     uint32_t tau = KEY_NONE, ties = 0;           // the kept set: keys above tau, and the first `ties` on it
     double target = -1.0;
     int found;
 
     if (s.greedy) {
-        for (int g = threadIdx.x; g < groups; g += ROW_THREADS)
-            if (top[g] == best) atomicMin(&S.group, g);
+        for (int g = threadIdx.x; g < groups; g += THREADS)
+            if (top[g] == best) atomicMin(&S.pick, g);
         __syncthreads();
-        found = S.group;
+        found = S.pick;
         tau = best - 1;
         if (threadIdx.x == 0) S.base = 0.0;
         __syncthreads();
     } else {
         if (massed)
-            for (int g = threadIdx.x; g < groups; g += ROW_THREADS) mass[g] = top[g] > KEY_NONE ? mass[g] * mass_of(value_of(top[g]), m, s.c) : 0.0;
-        if (s.k || s.p_on || s.m_on) {
+            for (int g = threadIdx.x; g < groups; g += THREADS) mass[g] = top[g] > KEY_NONE ? mass[g] * mass_of(value_of(top[g]), m, s.c) : 0.0;
+        if (filtered) {
             // Nothing below `low` is kept, nor counts in what top-p shares out.  (With top-k, top-p shares out the mass of the k first, also of
             // those that min-p drops, so min-p gives no bound there.)
             uint32_t low = KEY_LOWEST;
@@ -413,24 +661,90 @@ template <int XD> __global__ void __launch_bounds__(ROW_THREADS) k_sample_row(Sa
                 return max(low, min(best, max(key_of(f), KEY_LOWEST + 2) - 2));
             };
             if (s.m_on && !(s.k && s.p_on)) low = bound(m + log2(fmin(s.min_p, 1.0)) / s.c);
-            if (s.k && s.k <= groups) {          // k groups reach the k-th largest of their maxima, so k actions do
-                uint32_t t;
-                uint64_t a;
-                auto each = [&](auto take) {
-                    for (int g = threadIdx.x; g < groups; g += ROW_THREADS) take(top[g], [] { return 1ull; });
-                };
-                if (find_threshold(each, low, best, (uint64_t)s.k, S, &t, &a)) low = t;
+            if (s.k) {                           // each wave takes every W-th group: if q = k / W of them reach a value in every wave, k actions do
+                const int q = (s.k + W - 1) / W;
+                uint32_t t = 0;
+                if (q <= groups / W) {
+                    for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+                        int c = 0;
+                        for (int g = wave + lane * W; g - lane * W < groups; g += THREADS) c += __popcll(__ballot(g < groups && top[g] >= (t | bit)));
+                        if (c >= q) t |= bit;
+                    }
+                }
+                t = ~block_max<W>(~t, S.wave_u32);
+                low = max(low, t);
             }
-            double total = 0.0;
+            double all = 0.0;
             if (massed) {
-                __syncthreads();
-                for (int g = threadIdx.x; g < groups; g += ROW_THREADS) total += mass[g];
-                total = block_sum<ROW_WAVES>(total, S.wave_f64);
-                // the actions below (1 - p) of the mean mass have less than (1 - p) of the total together
-                low = bound(m + log2((1.0 - s.top_p) * total / A.v) / s.c);
+                for (int g = threadIdx.x; g < groups; g += THREADS) all += mass[g];
+                all = block_total<W>(all, S.wave_f64);
+                // Actions of a mass below b have less than (1 - p) of the total together if the groups' masses, each at most 128 b, do: then none of
+                // them is kept.  True for b = (1 - p) of the mean mass; the waves try 4, 16, ... times that.
+                const double rest = (1.0 - s.top_p) * all * (1.0 - 1e-9);
+                double b = rest / ((double)groups * GROUP);
+                uint32_t good = 0;
+                if (s.p_on) {
+#pragma unroll
+                    for (int i = 0; i < 16 / W; ++i) {
+                        const int step = wave * (16 / W) + i + 1;
+                        const double most = ldexp(b, 2 * step) * GROUP;
+                        double sum = 0.0;
+                        for (int g = lane; g < groups; g += 64) sum += fmin(mass[g], most);
+                        if (total(sum) < rest) good = step;
+                    }
+                    good = block_max<W>(good, S.wave_u32);
+                    low = bound(m + (log2(b) + 2.0 * good) / s.c);
+                }
             }
-            // every wave owns a run of the row and walks over the groups of it that reach `low`, in order
-            const int steps = (groups + 3) / 4, i0 = (int)((int64_t)steps * wave / ROW_WAVES), i1 = (int)((int64_t)steps * (wave + 1) / ROW_WAVES);
+            // The actions from `low` on, in their order: every wave owns a run of the groups, walks over those that reach `low`, sixteen lanes each,
+            // and appends to a segment of its own.
+            const int run0 = (int)((int64_t)groups * wave / W), run1 = (int)((int64_t)groups * (wave + 1) / W);
+            int count = 0;
+            for (int g0 = run0; g0 < run1; g0 += 64) {
+                uint64_t reach = __ballot(g0 + lane < run1 && top[min(g0 + lane, groups - 1)] >= low);
+                while (reach) {
+                    int mine = -1;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (reach) {
+                            const int bit = __ffsll((unsigned long long)reach) - 1;
+                            reach &= reach - 1;
+                            if (lane >> 4 == i) mine = g0 + bit;
+                        }
+                    float x[8];
+                    const int at = mine * GROUP + (lane & 15) * 8;
+                    if (mine >= 0) load_eight<XD>(A, xo, ao, at, x);
+                    uint32_t c = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (mine >= 0 && key_of(x[j]) >= low) c |= 1u << j;
+                    const uint32_t n = (uint32_t)__popc(c), upto = scan(n);
+                    int to = count + (int)(upto - n);
+                    count += (int)lane_of(upto, 63);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (c >> j & 1) {
+                            if (to < SEG) {
+                                R.x[wave * SEG + to] = x[j];
+                                R.index[wave * SEG + to] = at + j;
+                            }
+                            ++to;
+                        }
+                }
+            }
+            if (count > SEG && lane == 0) R.overflow = 1;
+            __syncthreads();
+            if (!R.overflow) {
+                float x[N];
+#pragma unroll
+                for (int j = 0; j < N; ++j) x[j] = lane * N + j < count ? R.x[wave * SEG + lane * N + j] : -INFINITY;
+                const int at = pick<XD, W, N>(x, s, u, A.v, best, low, massed ? all : 0.0, S);
+                if (threadIdx.x == 0) A.action[row] = at >= 0 ? R.index[at] : -1;
+                return;
+            }
+
+            // Too many for the registers: the same steps with the row read again for each.  Every wave walks over its run, four groups at a time.
+            const int steps = (groups + 3) / 4, i0 = (int)((int64_t)steps * wave / W), i1 = (int)((int64_t)steps * (wave + 1) / W);
             const uint32_t need = low;
             auto walk = [&](auto take) {
                 for (int i = i0; i < i1; ++i) {
@@ -445,19 +759,18 @@ template <int XD> __global__ void __launch_bounds__(ROW_THREADS) k_sample_row(Sa
                     take(g, q, x);
                 }
             };
-            // masses as integers: at most 2^50 each, their sum below 2^63
-            const double to_int = ldexp(1.0, min(50, 62 - (32 - __clz(A.v))));
-            auto int_mass = [&](float x) { return (uint64_t)(mass_of(x, m, s.c) * to_int + 0.5); };
+            const double scale = int_scale(A.v);
+            auto mass_int = [&](float x) { return int_mass(mass_of(x, m, s.c), scale); };
             uint64_t above;
             if (s.k) {
                 uint32_t t;
                 auto each = [&](auto take) {
                     walk([&](int, bool, const float *x) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) take(key_of(x[j]), [] { return 1ull; });
+                        for (int j = 0; j < 8; ++j) take(key_of(x[j]), x[j], [] { return 1ull; });
                     });
                 };
-                if (find_threshold(each, low, best, (uint64_t)s.k, S, &t, &above)) {
+                if (find_threshold(each, low, best, (uint64_t)s.k, ENDS, S, &t, &above)) {
                     tau = t;
                     ties = (uint32_t)(s.k - above);
                 }
@@ -465,30 +778,30 @@ template <int XD> __global__ void __launch_bounds__(ROW_THREADS) k_sample_row(Sa
             if (s.p_on) {
                 const uint32_t lowest = tau > KEY_NONE ? tau : low;
                 double limit;
-                if (massed) limit = s.top_p * total * to_int;
+                if (massed) limit = s.top_p * all * scale;
                 else {
                     uint64_t sum = 0;
                     walk([&](int, bool, const float *x) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
                             const uint32_t key = key_of(x[j]);
-                            if (key > tau && key >= lowest) sum += int_mass(x[j]);
+                            if (key > tau && key >= lowest) sum += mass_int(x[j]);
                         }
                     });
-                    sum = block_sum_u64(sum, S);
-                    if (tau > KEY_NONE) sum += ties * int_mass(value_of(tau));
+                    sum = block_total<W>(sum, (uint64_t *)S.wave_u64);
+                    if (tau > KEY_NONE) sum += ties * mass_int(value_of(tau));
                     limit = s.top_p * (double)sum;
                 }
-                const uint64_t amount = max((uint64_t)1, (uint64_t)ceil(limit));
+                const uint64_t amount = (uint64_t)fmax(1.0, ceil(limit));
                 uint32_t t;
                 auto each = [&](auto take) {
                     walk([&](int, bool, const float *x) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) take(key_of(x[j]), [&] { return int_mass(x[j]); });
+                        for (int j = 0; j < 8; ++j) take(key_of(x[j]), x[j], [&] { return mass_int(x[j]); });
                     });
                 };
-                if (find_threshold(each, lowest, best, amount, S, &t, &above)) {
-                    const uint64_t one = int_mass(value_of(t));
+                if (find_threshold(each, lowest, best, amount, ENDS, S, &t, &above)) {
+                    const uint64_t one = max((uint64_t)1, mass_int(value_of(t)));
                     const uint32_t r = (uint32_t)min((amount - above + one - 1) / one, (uint64_t)A.v);
                     if (t > tau) {
                         tau = t;
@@ -497,26 +810,27 @@ template <int XD> __global__ void __launch_bounds__(ROW_THREADS) k_sample_row(Sa
                 }
             }
             // what is kept of every group, and how many actions on the threshold come before it
-            int on = 0;
-            walk([&](int, bool, const float *x) {
+            uint32_t on = 0;
+            if (tau > KEY_NONE)
+                walk([&](int, bool, const float *x) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) on += key_of(x[j]) == tau;
-            });
-            if (tau <= KEY_NONE) on = 0;
-            on = (int)wave_sum_u64((uint64_t)on);
+                    for (int j = 0; j < 8; ++j) on += key_of(x[j]) == tau;
+                });
+            on = total(on);
             __syncthreads();
-            if (lane == 0) S.wave_u32[wave] = (uint32_t)on;
-            for (int g = threadIdx.x; g < groups; g += ROW_THREADS) mass[g] = 0.0;
+            if (lane == 0) S.wave_u32[wave] = on;
+            for (int g = threadIdx.x; g < groups; g += THREADS) mass[g] = 0.0;
+            if (threadIdx.x == 0) S.pick = 0x7FFFFFFF;
             __syncthreads();
             uint32_t seen = 0;
             for (int i = 0; i < wave; ++i) seen += S.wave_u32[i];
             walk([&](int g, bool q, const float *x) {
-                int c = 0;
+                uint32_t c = 0;
+                if (tau > KEY_NONE)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) c += key_of(x[j]) == tau;
-                if (tau <= KEY_NONE) c = 0;
-                const int upto = wave_scan_int(c, lane);
-                uint32_t rank = seen + (uint32_t)(upto - c);
+                    for (int j = 0; j < 8; ++j) c += key_of(x[j]) == tau;
+                const uint32_t upto = scan(c);
+                uint32_t rank = seen + upto - c;
                 const uint32_t rank0 = rank;
                 double w = 0.0;
 #pragma unroll
@@ -529,32 +843,30 @@ template <int XD> __global__ void __launch_bounds__(ROW_THREADS) k_sample_row(Sa
                         if (!s.m_on || wj >= s.min_p || key == best) w += wj;
                     }
                 }
-#pragma unroll
-                for (int d = 8; d; d >>= 1) w += __shfl_xor(w, d, 16);
-                if (q && (lane & 15) == 0) {
+                w = sum16(w);
+                const uint32_t first = (uint32_t)__shfl((int)rank0, lane & 48, 64);
+                if (q && (lane & 15) == 15) {
                     mass[g] = w;
-                    top[g] = rank0;
+                    top[g] = first;
                 }
-                seen += (uint32_t)__shfl(upto, 63, 64);
+                seen += lane_of(upto, 63);
             });
         }
         __syncthreads();
         // the group that the draw falls into: every thread adds up a run of groups, then the runs
-        const int per = (groups + ROW_THREADS - 1) / ROW_THREADS, g0 = min(groups, (int)threadIdx.x * per), g1 = min(groups, g0 + per);
+        const int per = (groups + THREADS - 1) / THREADS, g0 = min(groups, (int)threadIdx.x * per), g1 = min(groups, g0 + per);
         double own = 0.0;
         for (int g = g0; g < g1; ++g) own += mass[g];
-        const double sum = wave_scan(own, lane);
+        const double sum = scan(own);
         if (lane == 63) S.wave_f64[wave] = sum;
         __syncthreads();
-        double before = 0.0, all = 0.0;
+        double cum = sum - own, everything = 0.0;
 #pragma unroll
-        for (int i = 0; i < ROW_WAVES; ++i) {
-            before += i < wave ? S.wave_f64[i] : 0.0;
-            all += S.wave_f64[i];
+        for (int i = 0; i < W; ++i) {
+            cum += i < wave ? S.wave_f64[i] : 0.0;
+            everything += S.wave_f64[i];
         }
-        before += sum - own;
-        target = A.u[row] * all;
-        double cum = before;
+        target = u * everything;
         int mine = 0x7FFFFFFF, last = -1;
         double base = 0.0;
         for (int g = g0; g < g1; ++g) {
@@ -565,10 +877,10 @@ template <int XD> __global__ void __launch_bounds__(ROW_THREADS) k_sample_row(Sa
             }
             cum += mass[g];
         }
-        if (mine != 0x7FFFFFFF) atomicMin(&S.group, mine);
+        if (mine != 0x7FFFFFFF) atomicMin(&S.pick, mine);
         if (threadIdx.x == 0) S.bin = -1;
         __syncthreads();
-        found = S.group;
+        found = S.pick;
         if (found == mine && mine != 0x7FFFFFFF) S.base = base;
         if (found == 0x7FFFFFFF && last >= 0) atomicMax(&S.bin, last);
         __syncthreads();
@@ -580,8 +892,7 @@ template <int XD> __global__ void __launch_bounds__(ROW_THREADS) k_sample_row(Sa
     if (wave) return;
     // inside the group: two actions a lane, in order
     float x2[2];
-    uint32_t key[2];
-    int c = 0;
+    uint32_t key[2], c = 0;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int at = found * GROUP + lane * 2 + j;
@@ -589,8 +900,8 @@ template <int XD> __global__ void __launch_bounds__(ROW_THREADS) k_sample_row(Sa
         key[j] = key_of(x2[j]);
         c += key[j] == tau && tau > KEY_NONE;
     }
-    uint32_t rank = wave_scan_int(c, lane) - c;
-    if (!s.greedy && (s.k || s.p_on || s.m_on)) rank += top[found];
+    uint32_t rank = scan(c) - c;
+    if (!s.greedy && filtered) rank += top[found];
     bool kept[2];
     double w[2];
 #pragma unroll
@@ -603,7 +914,7 @@ template <int XD> __global__ void __launch_bounds__(ROW_THREADS) k_sample_row(Sa
             w[j] = 0.0;
         }
     }
-    const double upto = S.base + wave_scan(w[0] + w[1], lane);
+    const double upto = S.base + scan(w[0] + w[1]);
     const uint64_t any = __ballot(kept[0] || kept[1]), hit = __ballot(upto > target) & any;
     const int at = hit ? __ffsll((unsigned long long)hit) - 1 : 63 - __clzll((long long)any);
     if (lane == at) {
@@ -617,6 +928,9 @@ template <int XD> int launch(const SampleArgs &A, void *workspace, hipStream_t s
     const unsigned rows = (unsigned)A.n;
     if (A.v <= 128) hipLaunchKernelGGL((k_sample_wave<XD, 2>), dim3((rows + 3) / 4), dim3(256), 0, s, A);
     else if (A.v <= 512) hipLaunchKernelGGL((k_sample_wave<XD, 8>), dim3((rows + 3) / 4), dim3(256), 0, s, A);
+    else if (A.v <= 2048) hipLaunchKernelGGL((k_sample_block<XD, 4>), dim3(rows), dim3(256), 0, s, A);
+    else if (A.v <= 4096) hipLaunchKernelGGL((k_sample_block<XD, 8>), dim3(rows), dim3(512), 0, s, A);
+    else if (A.v <= BLOCK_V) hipLaunchKernelGGL((k_sample_block<XD, 16>), dim3(rows), dim3(1024), 0, s, A);
     else {
         const int groups = (A.v + GROUP - 1) / GROUP;
         double *mass = (double *)workspace;
@@ -632,10 +946,13 @@ template <int XD> int launch(const SampleArgs &A, void *workspace, hipStream_t s
             if (A.top_p_of) B.top_p_of = A.top_p_of + r;
             if (A.min_p_of) B.min_p_of = A.min_p_of + r;
             B.action = A.action + r;
-            hipLaunchKernelGGL((k_sample_groups<XD>), dim3((A.v + 2047) / 2048, (unsigned)B.n), dim3(256), 0, s, B, groups, mass + r * groups, top + r * groups);
+            const double *row_mass = mass + r * groups;
+            const uint32_t *row_top = top + r * groups;
+            hipLaunchKernelGGL((k_sample_groups<XD>), dim3((A.v + 2047) / 2048, (unsigned)B.n), dim3(256), 0, s, B, groups, (double *)row_mass, (uint32_t *)row_top);
             MZ_LAUNCH_CHECK("k_sample_groups");
-            hipLaunchKernelGGL((k_sample_row<XD>), dim3((unsigned)B.n), dim3(ROW_THREADS), (size_t)groups * 12, s, B, groups, (const double *)(mass + r * groups),
-                               (const uint32_t *)(top + r * groups));
+            // up to a row per CU: sixteen waves each; more rows: eight waves each, so that a CU works on two
+            if (A.n <= 256) hipLaunchKernelGGL((k_sample_row<XD, 16, 8>), dim3((unsigned)B.n), dim3(1024), (size_t)groups * 12, s, B, groups, row_mass, row_top);
+            else hipLaunchKernelGGL((k_sample_row<XD, 8, 8>), dim3((unsigned)B.n), dim3(512), (size_t)groups * 12, s, B, groups, row_mass, row_top);
             MZ_LAUNCH_CHECK("k_sample_row");
         }
     }
@@ -649,7 +966,7 @@ constexpr int64_t MAX_N = (1 << 22) - 1;
 
 extern "C" int64_t mz_sample_actions_workspace_bytes(int64_t n, int64_t v) {
     if (n < 0 || n > MAX_N || v < 1 || v > MAX_V) return -1;
-    return v <= 512 ? 0 : std::max<int64_t>(n, 1) * ((v + GROUP - 1) / GROUP) * 12;
+    return v <= BLOCK_V ? 0 : std::max<int64_t>(n, 1) * ((v + GROUP - 1) / GROUP) * 12;
 }
 
 extern "C" int mz_sample_actions(const mz_sample_args *a, void *workspace, int64_t workspace_bytes, void *stream) {

@@ -66,7 +66,7 @@ def _check(x, u, **kw):
 SETTINGS = [dict(), dict(temperature=0.0), dict(temperature=0.25), dict(top_k=1), dict(top_k=5), dict(top_p=0.9), dict(top_p=0.3, temperature=1.7), dict(min_p=0.05),
             dict(top_k=40, top_p=0.8, temperature=0.7), dict(top_k=300, top_p=0.95, min_p=0.01), dict(top_p=0.97, min_p=0.2), dict(top_p=0.0), dict(min_p=1.0),
             dict(top_k=10 ** 9, top_p=0.999), dict(top_k=2500, top_p=0.5, temperature=2.0), dict(top_p=0.999999, temperature=3.0)]
-SHAPES = [(1, 1), (5, 2), (3, 63), (9, 64), (64, 65), (5, 128), (5, 129), (7, 500), (4, 512), (5, 513), (3, 1000), (6, 2047), (3, 2049), (5, 5003), (3, 32768), (2, 100003), (2, 131072)]
+SHAPES = [(1, 1), (5, 2), (3, 63), (9, 64), (64, 65), (5, 128), (5, 129), (7, 500), (4, 512), (5, 513), (3, 1000), (6, 2047), (3, 2048), (3, 2049), (4, 4096), (3, 4097), (5, 5003), (2, 8192), (3, 8193), (3, 32768), (2, 100003), (2, 131072)]
 
 
 @pytest.mark.parametrize("kw", SETTINGS, ids=str)
@@ -98,7 +98,7 @@ def test_boards_of_legal_moves(kw):
     assert got[7].item() == 64 and got[8].item() == 63
 
 
-@pytest.mark.parametrize("v", [65, 500, 1024, 40000])
+@pytest.mark.parametrize("v", [65, 500, 1024, 4096, 6000, 40000])
 def test_equal_logits_go_to_the_lower_index(v):
     g = torch.Generator(device="cuda").manual_seed(v)
     x = torch.zeros(8, v, device="cuda")
@@ -116,7 +116,7 @@ def test_equal_logits_go_to_the_lower_index(v):
         _check(x, u, top_p=p, top_k=v // 2)
 
 
-@pytest.mark.parametrize("v", [65, 500, 3000, 50000])
+@pytest.mark.parametrize("v", [65, 500, 1500, 3000, 7000, 50000])
 def test_settings_of_their_own_for_every_row(v):
     g = torch.Generator(device="cuda").manual_seed(v + 1)
     n = 24
@@ -131,7 +131,7 @@ def test_settings_of_their_own_for_every_row(v):
     _check(x, _uniforms(n, 2), top_p=p)
 
 
-@pytest.mark.parametrize("v", [65, 500, 3000, 50000])
+@pytest.mark.parametrize("v", [65, 500, 1500, 3000, 7000, 50000])
 def test_infinities_nan_and_extreme_logits(v):
     x = torch.zeros(9, v, device="cuda")
     x[0, 3] = math.nan
@@ -153,7 +153,7 @@ def test_infinities_nan_and_extreme_logits(v):
         _check(x[:7], u[:7], temperature=t)
 
 
-@pytest.mark.parametrize("v", [65, 600])
+@pytest.mark.parametrize("v", [65, 600, 9000])
 def test_uniforms_outside_their_range(v):
     from muzero_amd.policy import sample_actions
     x = torch.zeros(4, v, device="cuda")
@@ -173,12 +173,23 @@ def test_frequencies_follow_the_distribution():
     assert bool((got[1:] >= got[:-1]).all())
 
 
+@pytest.mark.parametrize("kw", SETTINGS, ids=str)
+@pytest.mark.parametrize("v, dtype", [(9000, F32), (20011, BF16)], ids=str)
+def test_more_rows_than_the_card_has_cus(v, dtype, kw):
+    x = (2.5 * torch.randn(300, v, device="cuda", generator=torch.Generator(device="cuda").manual_seed(v))).to(dtype)
+    from muzero_amd.policy import sample_actions
+    u = _uniforms(300, 12)
+    got = sample_actions(x, u, **kw)
+    at = list(range(0, 300, 13))
+    assert got[at].tolist() == _want(x[at], u[at], **kw)
+
+
 def test_many_rows_and_the_largest_vocabulary():
     g = torch.Generator(device="cuda").manual_seed(9)
     x = torch.randn(1, 2 ** 19, device="cuda", generator=g) * 3
     for kw in (dict(), dict(top_p=0.9), dict(top_k=100, top_p=0.9), dict(top_k=20000)):
         _check(x, _uniforms(1, 1) + 0.37, **kw)
-    y = torch.randn(70000, 520, device="cuda", generator=g)      # more rows than one pair of launches takes
+    y = torch.randn(70000, 8200, device="cuda", generator=g, dtype=F32).to(F16)      # more rows than one pair of launches takes
     u = _uniforms(70000, 6)
     from muzero_amd.policy import sample_actions
     k = torch.randint(1, 50, (70000,), device="cuda", generator=g, dtype=torch.int32)

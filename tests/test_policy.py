@@ -61,7 +61,7 @@ def test_sample_actions_refuses_host_tensors():
 
 def _sample(L, **kw):
     P = 1 << 40                                   # never read: every call below is refused on the host
-    d = dict(logits=P, u=P, action=P, n=4, v=1000, logits_stride=1000, temperature=1.0, top_p=1.0)
+    d = dict(logits=P, u=P, action=P, n=4, v=10000, logits_stride=10000, temperature=1.0, top_p=1.0)
     d.update(kw)
     a = L.SampleArgs()
     for k, v in d.items():
@@ -89,10 +89,10 @@ def test_sample_arguments_are_checked_before_any_launch(kw, why):
 def test_sample_workspace_is_checked():
     from muzero_amd import _lib as L
     size = L.lib.mz_sample_actions_workspace_bytes
-    assert size(4, 512) == 0 and size(4, 513) == 4 * 5 * 12
+    assert size(4, 8192) == 0 and size(4, 8193) == 4 * 65 * 12
     for bad in ((-1, 65), (4, 0), (4, (1 << 19) + 1), (1 << 22, 65)):
         assert size(*bad) == -1
-    for ws, nbytes, why in ((None, 1 << 30, "workspace"), ((1 << 40) + 4, 1 << 30, "misaligned"), (1 << 40, size(4, 1000) - 1, "needed")):
+    for ws, nbytes, why in ((None, 1 << 30, "workspace"), ((1 << 40) + 4, 1 << 30, "misaligned"), (1 << 40, size(4, 10000) - 1, "needed")):
         with pytest.raises(L.MzError, match=why):
             L.call("mz_sample_actions", C.byref(_sample(L)), ws, nbytes, None)
     with pytest.raises(L.MzError, match="null arguments"):
