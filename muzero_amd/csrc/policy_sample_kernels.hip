@@ -16,6 +16,7 @@
 // reads only these again, takes the actions above the bound into registers (up to 4096 or 8192) and goes on as for a shorter row.
 #include <math.h>
 #include <algorithm>
+#include <type_traits>
 #include "numeric.h"
 
 namespace {
@@ -30,7 +31,7 @@ struct SampleArgs {
     const float *temperature_of, *top_p_of, *min_p_of;
     const int32_t *top_k_of;
     int32_t *action;
-    double temperature, top_p, min_p;
+    double temperature, c, top_p, min_p;   // c = log2(e) / temperature
     int64_t x_stride, allowed_stride, n;
     int v, top_k;
 };
@@ -51,7 +52,7 @@ __device__ __forceinline__ Setting setting_of(const SampleArgs &A, int64_t row) 
     const int k = A.top_k_of ? A.top_k_of[row] : A.top_k;
     s.k = k > 0 && k < A.v ? k : 0;
     s.greedy = !(T > 0.0) || s.k == 1;
-    s.c = s.greedy ? 0.0 : 1.4426950408889634 / T;
+    s.c = s.greedy ? 0.0 : A.temperature_of ? 1.4426950408889634 / T : A.c;
     s.p_on = (A.top_p_of ? (double)A.top_p_of[row] : A.top_p) < 1.0;   // a NaN is no limit
     s.m_on = s.min_p > 0.0;
     return s;
@@ -63,29 +64,43 @@ __device__ __forceinline__ uint32_t key_of(float x) {
     return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
+// (those of a 16-bit type end in bits that are 0 above zero and 1 below)
+template <int XD> constexpr int key_ends() { return XD == MZ_F32 ? 0 : XD == MZ_BF16 ? 16 : 13; }
 constexpr uint32_t KEY_NONE = 0x007FFFFFu;     // -inf: an action that cannot be played
 constexpr uint32_t KEY_LOWEST = 0x00800000u;   // the lowest finite value
 constexpr uint32_t KEY_INF = 0xFF800000u;      // +inf, and above it NaN: no distribution
 
 // 2^t for t <= 0: 2^round(t) times a polynomial at f = t - round(t) in [-1/2, 1/2], 1 + f q(f) with q the interpolation of (2^f - 1) / f at the
-// Chebyshev nodes of degree 9 (relative error 6e-16; 2^0 is 1 exactly)
-__device__ __forceinline__ double exp2_neg(double t) {
-    t = fmax(t, -1100.0);
-    const double r = rint(t), f = t - r;
-    double q = 7.070977866508138e-09;
-    q = fma(q, f, 1.0205905413765595e-07);
-    q = fma(q, f, 1.3215451633221434e-06);
-    q = fma(q, f, 1.5252672924850737e-05);
-    q = fma(q, f, 0.00015403530424776529);
-    q = fma(q, f, 0.0013333558200794592);
-    q = fma(q, f, 0.009618129107618665);
-    q = fma(q, f, 0.05550410866465167);
-    q = fma(q, f, 0.24022650695910075);
-    q = fma(q, f, 0.6931471805599462);
-    q = fma(q, f, 1.0);
-    return ldexp(q, (int)r);
+// Chebyshev nodes (2^0 is 1 exactly): of degree 9, relative error 6e-16, or where FINE is false of degree 7, 2e-12.  Adding 1.5 2^52 rounds t and
+// leaves the integer in the low word.  Below 2^-1000 the answer is 2^-1000: next to the row's best, whose mass is 1, nothing.
+template <bool FINE> __device__ __forceinline__ double exp2_neg(double t) {
+    t = fmax(t, -1000.0);
+    const double big = 6755399441055744.0, r = t + big, f = t - (r - big);
+    double q;
+    if (FINE) {
+        q = 7.070977866508138e-09;
+        q = fma(q, f, 1.0205905413765595e-07);
+        q = fma(q, f, 1.3215451633221434e-06);
+        q = fma(q, f, 1.5252672924850737e-05);
+        q = fma(q, f, 0.00015403530424776529);
+        q = fma(q, f, 0.0013333558200794592);
+        q = fma(q, f, 0.009618129107618665);
+        q = fma(q, f, 0.05550410866465167);
+        q = fma(q, f, 0.24022650695910075);
+        q = fma(q, f, 0.6931471805599462);
+    } else {
+        q = 1.325080551750225e-06;
+        q = fma(q, f, 1.5303700711365693e-05);
+        q = fma(q, f, 0.00015403475186530786);
+        q = fma(q, f, 0.0013333478473685416);
+        q = fma(q, f, 0.00961812913523614);
+        q = fma(q, f, 0.055504109063258665);
+        q = fma(q, f, 0.24022650695888503);
+        q = fma(q, f, 0.6931471805568324);
+    }
+    return ldexp(fma(q, f, 1.0), (int)(uint32_t)__double_as_longlong(r));
 }
-__device__ __forceinline__ double mass_of(float x, double m, double c) { return exp2_neg(((double)x - m) * c); }
+template <bool FINE = true> __device__ __forceinline__ double mass_of(float x, double m, double c) { return exp2_neg<FINE>(((double)x - m) * c); }
 
 // ---- reductions and scans over a wave in registers: rows of 16 lanes by shifts, then across the rows (lanes that get nothing add 0) ----------
 template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false); }
@@ -130,38 +145,19 @@ __device__ __forceinline__ double sum16(double v) {   // in the last of 16 lanes
 }
 __device__ __forceinline__ uint64_t lanes_below(int lane) { return lane ? ~0ull >> (64 - lane) : 0ull; }
 
-// ---- up to 512 actions: one wave per row, action j = 64 k + lane ---------------------------------------------------------------------
-template <int XD, int E> __global__ void __launch_bounds__(256) k_sample_wave(SampleArgs A) {
+// ---- up to 64 E values in one wave's registers, the i-th of them in x[i / 64] of lane i % 64 (-inf: none) ------------------------------------
+// The answer's i.  top: the largest key.  all: the mass that top-p shares out, if it is known (> 0).  Thresholds are found among the bits in which the
+// keys differ, for top-k one at a time, for top-p by parting the range into WAYS (4 where the wave is alone: three sums at once take little longer
+// than one; 2 where many waves share the CU: 4096 x 65 f32, top-p 0.9: 15.0 us against 20.6).
+template <int XD, int E, int WAYS> __device__ __forceinline__ int wave_pick(const float *x, const Setting &s, double u, uint32_t top, double all) {
     const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= A.n) return;
-    const Setting s = setting_of(A, row);
-    const int64_t xo = row * A.x_stride, ao = row * A.allowed_stride;
-    const uint64_t board = A.board ? A.board[row] : 0;
-    float x[E];
     uint32_t key[E];
-    uint32_t top = 0;
 #pragma unroll
-    for (int k = 0; k < E; ++k) {
-        const int j = k * 64 + lane;
-        bool ok = j < A.v;
-        if (ok && A.allowed) ok = A.allowed[ao + j] != 0;
-        if (ok && A.board) ok = j < 64 ? (board >> j) & 1 : board == 0;
-        x[k] = ok ? load_one<XD>(A.x, xo + j) : -INFINITY;
-        key[k] = x[k] != x[k] ? 0xFFFFFFFFu : key_of(x[k]);
-        top = max(top, key[k]);
-    }
-    top = wave_max_u32(top);
-    if (top <= KEY_NONE || top >= KEY_INF || s.bad) {
-        if (lane == 0) A.action[row] = -1;
-        return;
-    }
+    for (int k = 0; k < E; ++k) key[k] = key_of(x[k]);
     // the kept set: keys above tau, and the first `ties` on it
     uint32_t tau = KEY_NONE;
     int ties = 0;
     double w[E];
-#pragma unroll
-    for (int k = 0; k < E; ++k) w[k] = 0.0;
     if (s.greedy) {
         tau = top;
         ties = 1;
@@ -171,42 +167,69 @@ template <int XD, int E> __global__ void __launch_bounds__(256) k_sample_wave(Sa
         const double m = (double)value_of(top);
 #pragma unroll
         for (int k = 0; k < E; ++k) w[k] = key[k] > KEY_NONE ? mass_of(x[k], m, s.c) : 0.0;
-        if (s.k) {   // the largest tau that at least k keys reach, bit by bit from the top
-            uint32_t t = 0;
-            for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+        constexpr int ENDS = key_ends<XD>();
+        uint32_t least = 0xFFFFFFFFu;
+        int there = 0;
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            if (key[k] > KEY_NONE) least = min(least, key[k]);
+            there += __popcll(__ballot(key[k] > KEY_NONE));
+        }
+        least = ~wave_max_u32(~least);
+        if (s.k && s.k < there) {   // the largest tau that at least k keys reach
+            const uint32_t differ = least ^ top;
+            uint32_t bit = differ ? 0x80000000u >> __clz((int)differ) : 0, t = differ ? top & ~(bit | (bit - 1)) : top;
+            for (; bit >> ENDS; bit >>= 1) {
                 int c = 0;
 #pragma unroll
                 for (int k = 0; k < E; ++k) c += __popcll(__ballot(key[k] >= (t | bit)));
                 if (c >= s.k) t |= bit;
             }
-            if (t > KEY_NONE) {
-                int above = 0;
+            tau = 0xFFFFFFFFu;
+            int above = 0;
 #pragma unroll
-                for (int k = 0; k < E; ++k) above += __popcll(__ballot(key[k] > t));
-                tau = t;
-                ties = s.k - above;
-            }
+            for (int k = 0; k < E; ++k)
+                if (key[k] >= t) tau = min(tau, key[k]);
+            tau = ~wave_max_u32(~tau);
+#pragma unroll
+            for (int k = 0; k < E; ++k) above += __popcll(__ballot(key[k] > tau));
+            ties = s.k - above;
         }
         if (s.p_on) {   // the lowest tau above which less than p of the mass lies
-            const double w_tau = tau > KEY_NONE ? mass_of(value_of(tau), m, s.c) : 0.0;
-            double all = 0.0;
-            uint32_t lo = 0xFFFFFFFFu, hi = top;
+            double sum = 0.0;
 #pragma unroll
-            for (int k = 0; k < E; ++k) {
-                all += key[k] > tau ? w[k] : 0.0;
-                if (key[k] > KEY_NONE && key[k] >= tau) lo = min(lo, key[k]);
-            }
-            all = total(all) + (tau > KEY_NONE ? ties * w_tau : 0.0);
-            const double limit = s.top_p * all;
-            lo = ~wave_max_u32(~lo);             // the answer lies in [lo, hi]: the least key that can be kept, and the largest, above which nothing is
+            for (int k = 0; k < E; ++k) sum += key[k] > tau ? w[k] : 0.0;
+            sum = total(sum) + (tau > KEY_NONE ? ties * mass_of(value_of(tau), m, s.c) : 0.0);
+            const double limit = s.top_p * (all > 0.0 ? all : sum);
+            // the answer lies in [lo, hi]: the least key that can be kept, and the largest, above which nothing is (in steps of 2^ENDS, which part all keys)
+            uint32_t lo = max(least, tau) >> ENDS, hi = top >> ENDS;
             while (lo < hi) {
-                const uint32_t mid = lo + (hi - lo) / 2;
-                double above = 0.0;
+                const uint32_t step = max(1u, (hi - lo + 1) / WAYS);
+                uint32_t mid[WAYS - 1];
+                double over[WAYS - 1];
 #pragma unroll
-                for (int k = 0; k < E; ++k) above += key[k] > mid ? w[k] : 0.0;
-                if (total(above) < limit) hi = mid;
-                else lo = mid + 1;
+                for (int i = 0; i < WAYS - 1; ++i) {
+                    mid[i] = min(hi, lo + step * (i + 1) - 1);
+                    const uint32_t edge = mid[i] << ENDS | ((1u << ENDS) - 1);
+                    over[i] = 0.0;
+#pragma unroll
+                    for (int k = 0; k < E; ++k) over[i] += key[k] > edge ? w[k] : 0.0;
+                }
+#pragma unroll
+                for (int i = 0; i < WAYS - 1; ++i) over[i] = scan(over[i]);
+                uint32_t from = lo;
+                bool done = false;
+#pragma unroll
+                for (int i = 0; i < WAYS - 1; ++i) {
+                    if (done) continue;
+                    if (lane_of(over[i], 63) < limit) {
+                        hi = mid[i];
+                        done = true;
+                    } else from = mid[i] + 1;
+                }
+                lo = min(from, hi);
             }
+            lo = ENDS ? (lo << ENDS) | (lo << ENDS & 0x80000000u ? 0 : (1u << ENDS) - 1) : lo;
             double above = 0.0;
             int on = 0;
 #pragma unroll
@@ -242,7 +265,7 @@ template <int XD, int E> __global__ void __launch_bounds__(256) k_sample_wave(Sa
             base = lane_of(part[k], 63);
         }
     }
-    const double target = A.u[row] * base;
+    const double target = u * base;
     int pick = -1, last = -1;
 #pragma unroll
     for (int k = 0; k < E; ++k) {
@@ -250,25 +273,61 @@ template <int XD, int E> __global__ void __launch_bounds__(256) k_sample_wave(Sa
         if (pick < 0 && hit) pick = k * 64 + __ffsll((unsigned long long)hit) - 1;
         if (keep[k]) last = k * 64 + 63 - __clzll((long long)keep[k]);
     }
-    if (lane == 0) A.action[row] = pick < 0 ? last : pick;
+    return pick < 0 ? last : pick;
 }
 
-// eight actions of a row; what lies behind its end or is not legal is -inf
-template <int XD> __device__ __forceinline__ void load_eight(const SampleArgs &A, int64_t xo, int64_t ao, int at, float *x) {
-    if (at + 8 <= A.v) {
-        const Words<XD, 8> p = load_words<XD, 8>(A.x, xo + at);
+// ---- up to 512 actions: one wave per row ---------------------------------------------------------------------------------------------
+template <int XD, int E> __global__ void __launch_bounds__(256) k_sample_wave(SampleArgs A) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= A.n) return;
+    const Setting s = setting_of(A, row);
+    const int64_t xo = row * A.x_stride, ao = row * A.allowed_stride;
+    const uint64_t board = A.board ? A.board[row] : 0;
+    float x[E];
+    uint32_t top = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = p.get(j);
-        if (A.allowed) {
-            const uint64_t ok = load_flags(A.allowed, ao + at);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = (ok >> j * 8) & 0xFF ? x[j] : -INFINITY;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = at + j < A.v && (!A.allowed || A.allowed[ao + at + j]) ? load_one<XD>(A.x, xo + at + j) : -INFINITY;
+    for (int k = 0; k < E; ++k) {
+        const int j = k * 64 + lane;
+        bool ok = j < A.v;
+        if (ok && A.allowed) ok = A.allowed[ao + j] != 0;
+        if (ok && A.board) ok = j < 64 ? (board >> j) & 1 : board == 0;
+        x[k] = ok ? load_one<XD>(A.x, xo + j) : -INFINITY;
+        top = max(top, x[k] != x[k] ? 0xFFFFFFFFu : key_of(x[k]));
     }
+    top = wave_max_u32(top);
+    if (top <= KEY_NONE || top >= KEY_INF || s.bad) {
+        if (lane == 0) A.action[row] = -1;
+        return;
+    }
+    const int pick = wave_pick<XD, E, 2>(x, s, A.u[row], top, 0.0);
+    if (lane == 0) A.action[row] = pick;
 }
+
+// eight actions of a row as they lie there (so that their loads can be under way while others are worked on)
+template <int XD> struct Eight {
+    Words<XD, 8> words;
+    uint64_t ok;                                 // a byte each; 0: behind the row's end or not legal, -inf
+    __device__ __forceinline__ void load(const SampleArgs &A, int64_t xo, int64_t ao, int at) {
+        if (at + 8 <= A.v) {
+            words = load_words<XD, 8>(A.x, xo + at);
+            ok = A.allowed ? load_flags(A.allowed, ao + at) : ~0ull;
+        } else {
+            words = {};
+            ok = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (at + j < A.v && (!A.allowed || A.allowed[ao + at + j])) {
+                    words.set(j, ((const MZ_GLOBAL typename Elem<XD>::T *)A.x)[xo + at + j]);
+                    ok |= 0xFFull << j * 8;
+                }
+        }
+    }
+    __device__ __forceinline__ void unpack(float *x) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = (ok >> j * 8) & 0xFF ? words.get(j) : -INFINITY;
+    }
+};
 
 // ---- what a workgroup of W waves does together -----------------------------------------------------------------------------------------
 template <int W> struct Shared {
@@ -315,7 +374,8 @@ template <int W> __device__ __forceinline__ int crossing_bin(Shared<W> &S, uint6
     if (lane == 63) S.wave_u64[wave] = sum;
     __syncthreads();
     uint64_t before = *above + sum - own;
-    for (int i = 0; i < wave; ++i) before += S.wave_u64[i];
+#pragma unroll
+    for (int i = 0; i < W; ++i) before += i < wave ? S.wave_u64[i] : 0;
     if (before < limit && before + own >= limit) {   // one thread at most
         int i = 0;
         while (before + h[0] < limit) {
@@ -335,10 +395,10 @@ template <int W> __device__ __forceinline__ int crossing_bin(Shared<W> &S, uint6
 
 // The lowest tau in [lo, hi] with (amount above tau) < limit, where `each` hands (key, value, function of the amount) of everything in the row to
 // its argument; *above = that amount.  False: all of it together stays below the limit.  Amounts are integers, so the order of the atomics does
-// not matter.  `lo` may be lowered by nothing; `ends` = bits of a key that its type leaves empty.
-// The first histogram has bins of equal width in the value, which few logits share; the up to 64 of the bin that reaches the limit are ranked in
-// registers.  More (equal logits): histograms over the keys' bits, each narrowing to one bin of the one before.
-template <int W, class EACH> __device__ __forceinline__ bool find_threshold(EACH each, uint32_t lo, uint32_t hi, uint64_t limit, int ends, Shared<W> &S, uint32_t *tau, uint64_t *above_out) {
+// not matter.  `guess` >= lo: where tau is looked for first; `ends` = bits of a key that its type leaves empty.
+// The first histogram, from `guess` on, has bins of equal width in the value, which few logits share; the up to 64 of the bin that reaches the limit
+// are ranked in registers.  More (equal logits), or tau below the guess: histograms over the keys' bits, each narrowing to one bin of the one before.
+template <int W, class EACH> __device__ __forceinline__ bool find_threshold(EACH each, uint32_t lo, uint32_t guess, uint32_t hi, uint64_t limit, int ends, Shared<W> &S, uint32_t *tau, uint64_t *above_out) {
     constexpr int BINS = Shared<W>::BINS, BITS = W == 4 ? 10 : W == 8 ? 11 : 12, FEW = Shared<W>::FEW;
     static_assert(1 << BITS == BINS, "a bin for each key of that many bits");
     const int lane = threadIdx.x & 63;
@@ -353,18 +413,18 @@ template <int W, class EACH> __device__ __forceinline__ bool find_threshold(EACH
         __syncthreads();
     };
     uint64_t above = 0;
-    const float xh = value_of(hi), width = xh - value_of(lo), scale = BINS / width;
-    if (((hi - lo) >> ends) >= BINS && scale > 0.0f && scale < 1e30f) {
+    const float xh = value_of(hi), width = xh - value_of(guess), scale = BINS / width;
+    if (((hi - guess) >> ends) >= BINS && scale > 0.0f && scale < 1e30f) {
         auto bin_of = [&](float x) { return min(BINS - 1, (int)((xh - x) * scale)); };
         clear();
         each([&](uint32_t key, float x, auto amount) {
-            if (key >= lo && key <= hi) atomicAdd(&S.hist[bin_of(x)], (unsigned long long)amount());
+            if (key >= guess && key <= hi) atomicAdd(&S.hist[bin_of(x)], (unsigned long long)amount());
         });
         __syncthreads();
         const int bin = crossing_bin(S, limit, &above);
-        if (bin < 0) return false;
-        each([&](uint32_t key, float x, auto amount) {
-            if (key >= lo && key <= hi && bin_of(x) == bin) {
+        if (bin < 0 && guess == lo) return false;
+        if (bin >= 0) each([&](uint32_t key, float x, auto amount) {
+            if (key >= guess && key <= hi && bin_of(x) == bin) {
                 const int i = atomicAdd(&S.few, 1);
                 if (i < FEW) {
                     S.few_key[i] = key;
@@ -374,7 +434,7 @@ template <int W, class EACH> __device__ __forceinline__ bool find_threshold(EACH
         });
         __syncthreads();
         const int few = S.few;
-        if (few <= FEW) {
+        if (bin >= 0 && few <= FEW) {
             const uint32_t key = lane < few ? S.few_key[lane] : 0;
             const uint64_t amount = lane < few ? (uint64_t)S.few_amount[lane] : 0;
             uint64_t over = above;
@@ -411,7 +471,6 @@ template <int W, class EACH> __device__ __forceinline__ bool find_threshold(EACH
         lo = hi - lo < (1u << shift) ? lo : hi - (1u << shift) + 1;
     }
 }
-template <int XD> constexpr int key_ends() { return XD == MZ_F32 ? 0 : XD == MZ_BF16 ? 16 : 13; }
 
 // masses as integers: at most 2^50 each, their sum over v actions below 2^63
 __device__ __forceinline__ double int_scale(int v) { return ldexp(1.0, min(50, 62 - (32 - __clz(v)))); }
@@ -427,11 +486,7 @@ template <int XD, int W, int N> __device__ __forceinline__ int pick(const float 
     const double m = (double)value_of(best);
     uint32_t tau = KEY_NONE, ties = 0;           // the kept set: keys above tau, and the first `ties` on it
     double w[N];
-    if (s.greedy) {
-        tau = best - 1;
-#pragma unroll
-        for (int j = 0; j < N; ++j) w[j] = 1.0;
-    } else {
+    {
 #pragma unroll
         for (int j = 0; j < N; ++j) w[j] = mass_of(x[j], m, s.c);
         uint64_t above;
@@ -450,7 +505,7 @@ template <int XD, int W, int N> __device__ __forceinline__ int pick(const float 
                 for (int j = 0; j < N; ++j) take(key_of(x[j]), x[j], [] { return 1ull; });
             };
             uint32_t t;
-            if (find_threshold(each, low, best, (uint64_t)s.k, ENDS, S, &t, &above)) {
+            if (find_threshold(each, low, low, best, (uint64_t)s.k, ENDS, S, &t, &above)) {
                 tau = t;
                 ties = (uint32_t)(s.k - above);
             }
@@ -477,7 +532,7 @@ template <int XD, int W, int N> __device__ __forceinline__ int pick(const float 
                 for (int j = 0; j < N; ++j) take(key_of(x[j]), x[j], [&] { return int_mass(w[j], scale); });
             };
             uint32_t t;
-            if (find_threshold(each, lowest, best, amount, ENDS, S, &t, &above)) {
+            if (find_threshold(each, lowest, lowest, best, amount, ENDS, S, &t, &above)) {
                 const uint64_t one = max((uint64_t)1, int_mass(mass_of(value_of(t), m, s.c), scale));
                 const uint32_t r = (uint32_t)min((amount - above + one - 1) / one, (uint64_t)v);
                 if (t > tau) {
@@ -498,7 +553,8 @@ template <int XD, int W, int N> __device__ __forceinline__ int pick(const float 
     if (threadIdx.x == 0) S.pick = 0x7FFFFFFF;
     __syncthreads();
     uint32_t rank = on_upto - on;
-    for (int i = 0; i < wave; ++i) rank += S.wave_u32[i];
+#pragma unroll
+    for (int i = 0; i < W; ++i) rank += i < wave ? S.wave_u32[i] : 0;
     double own = 0.0;
     uint32_t keep = 0;
 #pragma unroll
@@ -506,7 +562,7 @@ template <int XD, int W, int N> __device__ __forceinline__ int pick(const float 
         const uint32_t key = key_of(x[j]);
         bool kept = key > tau;
         if (key == tau && on) kept = rank++ < ties;
-        if (!s.greedy && s.m_on) kept = kept && (w[j] >= s.min_p || key == best);
+        if (s.m_on) kept = kept && (w[j] >= s.min_p || key == best);
         if (kept) {
             keep |= 1u << j;
             own += w[j];
@@ -521,7 +577,7 @@ template <int XD, int W, int N> __device__ __forceinline__ int pick(const float 
         cum += i < wave ? S.wave_f64[i] : 0.0;
         everything += S.wave_f64[i];
     }
-    const double target = s.greedy ? -1.0 : u * everything;
+    const double target = u * everything;
     int mine = -1, last = -1;
 #pragma unroll
     for (int j = 0; j < N; ++j)
@@ -550,13 +606,25 @@ template <int XD, int W> __global__ void __launch_bounds__(64 * W) k_sample_bloc
     const int64_t row = blockIdx.x;
     const Setting s = setting_of(A, row);
     float x[8];
-    load_eight<XD>(A, row * A.x_stride, row * A.allowed_stride, threadIdx.x * 8, x);
+    Eight<XD> e;
+    e.load(A, row * A.x_stride, row * A.allowed_stride, threadIdx.x * 8);
+    e.unpack(x);
     uint32_t best = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) best = max(best, x[j] != x[j] ? 0xFFFFFFFFu : key_of(x[j]));
     best = block_max<W>(best, S.wave_u32);
     if (best <= KEY_NONE || best >= KEY_INF || s.bad) {
         if (threadIdx.x == 0) A.action[row] = -1;
+        return;
+    }
+    if (s.greedy) {
+        if (threadIdx.x == 0) S.pick = 0x7FFFFFFF;
+        __syncthreads();
+#pragma unroll
+        for (int j = 7; j >= 0; --j)
+            if (key_of(x[j]) == best) atomicMin(&S.pick, (int)threadIdx.x * 8 + j);
+        __syncthreads();
+        if (threadIdx.x == 0) A.action[row] = S.pick;
         return;
     }
     const int at = pick<XD, W, 8>(x, s, A.u[row], A.v, best, KEY_LOWEST, 0.0, S);
@@ -571,32 +639,42 @@ constexpr int BLOCK_V = 8192;       // the longest row that one workgroup holds 
 // whether a row's total mass has to come from all of its actions
 __device__ __forceinline__ bool needs_mass(const Setting &s) { return !s.greedy && !s.k && (s.p_on || !s.m_on); }
 
-// a workgroup takes 2048 actions of one row, sixteen lanes a group
-template <int XD> __global__ void __launch_bounds__(256) k_sample_groups(SampleArgs A, int groups, double *mass, uint32_t *top) {
+// a workgroup takes TILES x 2048 actions of one row, sixteen lanes a group, the next tile's loads under way
+template <int XD, int TILES> __global__ void __launch_bounds__(256) k_sample_groups(SampleArgs A, int groups, double *mass, uint32_t *top) {
     const int64_t row = blockIdx.y;
-    const int at = blockIdx.x * 2048 + threadIdx.x * 8, g = at / GROUP;
     const Setting s = setting_of(A, row);
-    float x[8];
-    load_eight<XD>(A, row * A.x_stride, row * A.allowed_stride, at, x);   // behind the row's end: nothing is read
-    float m = -INFINITY;
-    bool nan = false;
+    const bool massed = needs_mass(s);
+    const int64_t xo = row * A.x_stride, ao = row * A.allowed_stride;
+    const int first = blockIdx.x * (TILES * 2048) + threadIdx.x * 8;
+    Eight<XD> e, e2;
+    e.load(A, xo, ao, first);                    // behind the row's end: nothing is read
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        m = fmaxf(m, x[j]);
-        nan |= x[j] != x[j];
-    }
-    const uint32_t key = lane_last16(max16(nan ? 0xFFFFFFFFu : key_of(m)));
-    const bool writes = (threadIdx.x & 15) == 15 && g < groups;
-    if (writes) top[row * groups + g] = key;
-    if (!needs_mass(s)) return;
-    double w = 0.0;
-    if (key > KEY_NONE && key < KEY_INF) {
-        const double md = (double)value_of(key);
+    for (int t = 0; t < TILES; ++t) {
+        const int at = first + t * 2048, g = at / GROUP;
+        if (t + 1 < TILES) e2.load(A, xo, ao, at + 2048);
+        float x[8], m = -INFINITY;
+        e.unpack(x);
+        bool nan = false;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w += mass_of(x[j], md, s.c);
+        for (int j = 0; j < 8; ++j) {
+            m = fmaxf(m, x[j]);
+            nan |= x[j] != x[j];
+        }
+        const uint32_t key = lane_last16(max16(nan ? 0xFFFFFFFFu : key_of(m)));
+        const bool writes = (threadIdx.x & 15) == 15 && g < groups;
+        if (writes) top[row * groups + g] = key;
+        if (massed) {
+            double w = 0.0;
+            if (key > KEY_NONE && key < KEY_INF) {
+                const double md = (double)value_of(key);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w += mass_of<false>(x[j], md, s.c);   // 2e-12 of a group's mass moves no draw that 1e-12 of the row would not
+            }
+            w = sum16(w);
+            if (writes) mass[row * groups + g] = w;
+        }
+        if (t + 1 < TILES) e = e2;
     }
-    w = sum16(w);
-    if (writes) mass[row * groups + g] = w;
 }
 
 // LDS of a row: its groups, then the actions that its bounds leave, SEG to each wave
@@ -605,7 +683,6 @@ template <int W, int N> struct RowShared {
     Shared<W> S;
     float x[W * SEG];
     int32_t index[W * SEG];
-    int overflow;
 };
 
 template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_sample_row(SampleArgs A, int groups, const double *mass_in, const uint32_t *top_in) {
@@ -627,10 +704,7 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
         if (massed) mass[g] = mass_in[row * groups + g];
         best = max(best, top[g]);
     }
-    if (threadIdx.x == 0) {
-        S.pick = 0x7FFFFFFF;
-        R.overflow = 0;
-    }
+    if (threadIdx.x == 0) S.pick = 0x7FFFFFFF;
     best = block_max<W>(best, S.wave_u32);
     if (best <= KEY_NONE || best >= KEY_INF || s.bad) {
         if (threadIdx.x == 0) A.action[row] = -1;
@@ -656,6 +730,7 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
             // Nothing below `low` is kept, nor counts in what top-p shares out.  (With top-k, top-p shares out the mass of the k first, also of
             // those that min-p drops, so min-p gives no bound there.)
             uint32_t low = KEY_LOWEST;
+            bool bounded = true;
             auto bound = [&](double x) {         // the key of a value a little below x
                 const float f = (float)(x - 1e-6 * (fabs(x) + fabs(m)));
                 return max(low, min(best, max(key_of(f), KEY_LOWEST + 2) - 2));
@@ -664,12 +739,26 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
             if (s.k) {                           // each wave takes every W-th group: if q = k / W of them reach a value in every wave, k actions do
                 const int q = (s.k + W - 1) / W;
                 uint32_t t = 0;
-                if (q <= groups / W) {
-                    for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
-                        int c = 0;
-                        for (int g = wave + lane * W; g - lane * W < groups; g += THREADS) c += __popcll(__ballot(g < groups && top[g] >= (t | bit)));
-                        if (c >= q) t |= bit;
+                bounded = q <= groups / W;
+                if (bounded) {
+                    constexpr int PER = MAX_V / GROUP / THREADS;
+                    uint32_t mine[PER];
+#pragma unroll
+                    for (int i = 0; i < PER; ++i) {
+                        const int g = wave + lane * W + i * THREADS;
+                        mine[i] = g < groups ? top[g] : 0;
                     }
+                    // the low bits stay 0: a little lower is a bound too
+                    if (groups <= THREADS) {
+                        for (uint32_t bit = 0x80000000u; bit > 0x2000; bit >>= 1)
+                            if ((int)__popcll(__ballot(mine[0] >= (t | bit))) >= q) t |= bit;
+                    } else
+                        for (uint32_t bit = 0x80000000u; bit > 0x2000; bit >>= 1) {
+                            int c = 0;
+#pragma unroll
+                            for (int i = 0; i < PER; ++i) c += (int)__popcll(__ballot(mine[i] >= (t | bit)));
+                            if (c >= q) t |= bit;
+                        }
                 }
                 t = ~block_max<W>(~t, S.wave_u32);
                 low = max(low, t);
@@ -696,28 +785,54 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
                     low = bound(m + (log2(b) + 2.0 * good) / s.c);
                 }
             }
-            // The actions from `low` on, in their order: every wave owns a run of the groups, walks over those that reach `low`, sixteen lanes each,
-            // and appends to a segment of its own.
+            // Every wave owns a run of the groups and walks over those that reach `need`, in order, sixteen lanes to a group, the loads of DEPTH times
+            // four groups under way together; `take` gets a lane's group (-1: none) and its eight actions, and says whether to go on.
             const int run0 = (int)((int64_t)groups * wave / W), run1 = (int)((int64_t)groups * (wave + 1) / W);
-            int count = 0;
-            for (int g0 = run0; g0 < run1; g0 += 64) {
-                uint64_t reach = __ballot(g0 + lane < run1 && top[min(g0 + lane, groups - 1)] >= low);
-                while (reach) {
-                    int mine = -1;
+            auto walk = [&](uint32_t need, auto take) {
+                constexpr int DEPTH = XD == MZ_F32 ? 3 : 4;   // what fits 128 registers
+                int g0 = run0 - 64;
+                uint64_t reach = 0;
+                for (;;) {
+                    Eight<XD> e[DEPTH];
+                    int mine[DEPTH];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (reach) {
-                            const int bit = __ffsll((unsigned long long)reach) - 1;
-                            reach &= reach - 1;
-                            if (lane >> 4 == i) mine = g0 + bit;
+                    for (int d = 0; d < DEPTH; ++d) {
+                        while (!reach && g0 + 64 < run1) {
+                            g0 += 64;
+                            reach = __ballot(g0 + lane < run1 && top[min(g0 + lane, groups - 1)] >= need);
                         }
-                    float x[8];
-                    const int at = mine * GROUP + (lane & 15) * 8;
-                    if (mine >= 0) load_eight<XD>(A, xo, ao, at, x);
+                        mine[d] = -1;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (reach) {
+                                const int bit = __ffsll((unsigned long long)reach) - 1;
+                                reach &= reach - 1;
+                                if (lane >> 4 == i) mine[d] = g0 + bit;
+                            }
+                        if (mine[d] >= 0) e[d].load(A, xo, ao, mine[d] * GROUP + (lane & 15) * 8);
+                        else {
+                            e[d].words = {};
+                            e[d].ok = 0;
+                        }
+                    }
+#pragma unroll
+                    for (int d = 0; d < DEPTH; ++d) {
+                        if (!__ballot(mine[d] >= 0)) return;
+                        float x[8];
+                        e[d].unpack(x);
+                        if (!take(mine[d], x)) return;
+                    }
+                }
+            };
+            // the actions from `low` on, in their order, each wave's in a segment of its own
+            int count = 0;
+            if (bounded)
+                walk(low, [&](int g, const float *x) {
                     uint32_t c = 0;
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        if (mine >= 0 && key_of(x[j]) >= low) c |= 1u << j;
+                        if (key_of(x[j]) >= low) c |= 1u << j;
+                    if (!__ballot(c)) return true;
                     const uint32_t n = (uint32_t)__popc(c), upto = scan(n);
                     int to = count + (int)(upto - n);
                     count += (int)lane_of(upto, 63);
@@ -726,15 +841,50 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
                         if (c >> j & 1) {
                             if (to < SEG) {
                                 R.x[wave * SEG + to] = x[j];
-                                R.index[wave * SEG + to] = at + j;
+                                R.index[wave * SEG + to] = g * GROUP + (lane & 15) * 8 + j;
                             }
                             ++to;
                         }
-                }
-            }
-            if (count > SEG && lane == 0) R.overflow = 1;
+                    return count <= SEG;
+                });
+            if (lane == 0) S.wave_u32[wave] = bounded ? (uint32_t)count : SEG + 1u;
             __syncthreads();
-            if (!R.overflow) {
+            int many = 0, most = 0, start[W + 1];
+            start[0] = 0;
+            const uint32_t of_wave = lane < W ? S.wave_u32[lane] : 0;
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const int c = (int)lane_of(of_wave, i);
+                most = max(most, c);
+                many += c;
+                start[i + 1] = many;
+            }
+            if (most <= SEG && many <= 512) {    // few: one wave goes on without the others
+                if (wave) return;
+                auto finish = [&](auto size) {
+                    constexpr int E = decltype(size)::value;
+                    int slot[E];
+                    float x[E];
+#pragma unroll
+                    for (int k = 0; k < E; ++k) {
+                        const int i = k * 64 + lane;
+                        slot[k] = i;
+#pragma unroll
+                        for (int j = 1; j < W; ++j) slot[k] = i >= start[j] ? j * SEG + i - start[j] : slot[k];
+                        x[k] = i < many ? R.x[slot[k]] : -INFINITY;
+                    }
+                    const int at = wave_pick<XD, E, 4>(x, s, u, best, massed ? all : 0.0);
+#pragma unroll
+                    for (int k = 0; k < E; ++k)
+                        if (at >= 0 && at >> 6 == k && (at & 63) == lane) A.action[row] = R.index[slot[k]];
+                };
+                if (many <= 64) finish(std::integral_constant<int, 1>());
+                else if (many <= 192) finish(std::integral_constant<int, 3>());
+                else finish(std::integral_constant<int, 8>());
+                return;
+            }
+            __syncthreads();                     // wave_u32 is used again
+            if (most <= SEG) {
                 float x[N];
 #pragma unroll
                 for (int j = 0; j < N; ++j) x[j] = lane * N + j < count ? R.x[wave * SEG + lane * N + j] : -INFINITY;
@@ -743,34 +893,28 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
                 return;
             }
 
-            // Too many for the registers: the same steps with the row read again for each.  Every wave walks over its run, four groups at a time.
-            const int steps = (groups + 3) / 4, i0 = (int)((int64_t)steps * wave / W), i1 = (int)((int64_t)steps * (wave + 1) / W);
-            const uint32_t need = low;
-            auto walk = [&](auto take) {
-                for (int i = i0; i < i1; ++i) {
-                    const int g = i * 4 + (lane >> 4);
-                    const bool q = g < groups && top[g] >= need;
-                    if (!__ballot(q)) continue;
-                    float x[8];
-                    if (q) load_eight<XD>(A, xo, ao, i * 512 + lane * 8, x);
-                    else
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) x[j] = -INFINITY;
-                    take(g, q, x);
-                }
-            };
+            // Too many for the registers: the same steps with the row read again for each.
             const double scale = int_scale(A.v);
             auto mass_int = [&](float x) { return int_mass(mass_of(x, m, s.c), scale); };
             uint64_t above;
             if (s.k) {
                 uint32_t t;
                 auto each = [&](auto take) {
-                    walk([&](int, bool, const float *x) {
+                    walk(low, [&](int, const float *x) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j) take(key_of(x[j]), x[j], [] { return 1ull; });
+                        return true;
                     });
                 };
-                if (find_threshold(each, low, best, (uint64_t)s.k, ENDS, S, &t, &above)) {
+                uint32_t guess = low;
+                if (!bounded) {                  // twice as far below the best as the least of the groups' maxima
+                    uint32_t least = 0xFFFFFFFFu;
+                    for (int g = threadIdx.x; g < groups; g += THREADS)
+                        if (top[g] > KEY_NONE) least = min(least, top[g]);
+                    least = ~block_max<W>(~least, S.wave_u32);
+                    guess = bound(m - 2.0 * (m - (double)value_of(least)));
+                }
+                if (find_threshold(each, low, guess, best, (uint64_t)s.k, ENDS, S, &t, &above)) {
                     tau = t;
                     ties = (uint32_t)(s.k - above);
                 }
@@ -781,12 +925,13 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
                 if (massed) limit = s.top_p * all * scale;
                 else {
                     uint64_t sum = 0;
-                    walk([&](int, bool, const float *x) {
+                    walk(lowest, [&](int, const float *x) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
                             const uint32_t key = key_of(x[j]);
                             if (key > tau && key >= lowest) sum += mass_int(x[j]);
                         }
+                        return true;
                     });
                     sum = block_total<W>(sum, (uint64_t *)S.wave_u64);
                     if (tau > KEY_NONE) sum += ties * mass_int(value_of(tau));
@@ -795,12 +940,13 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
                 const uint64_t amount = (uint64_t)fmax(1.0, ceil(limit));
                 uint32_t t;
                 auto each = [&](auto take) {
-                    walk([&](int, bool, const float *x) {
+                    walk(lowest, [&](int, const float *x) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j) take(key_of(x[j]), x[j], [&] { return mass_int(x[j]); });
+                        return true;
                     });
                 };
-                if (find_threshold(each, lowest, best, amount, ENDS, S, &t, &above)) {
+                if (find_threshold(each, lowest, lowest, best, amount, ENDS, S, &t, &above)) {
                     const uint64_t one = max((uint64_t)1, mass_int(value_of(t)));
                     const uint32_t r = (uint32_t)min((amount - above + one - 1) / one, (uint64_t)A.v);
                     if (t > tau) {
@@ -811,10 +957,12 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
             }
             // what is kept of every group, and how many actions on the threshold come before it
             uint32_t on = 0;
+            const uint32_t need = max(low, tau);
             if (tau > KEY_NONE)
-                walk([&](int, bool, const float *x) {
+                walk(need, [&](int, const float *x) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) on += key_of(x[j]) == tau;
+                    return true;
                 });
             on = total(on);
             __syncthreads();
@@ -823,8 +971,9 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
             if (threadIdx.x == 0) S.pick = 0x7FFFFFFF;
             __syncthreads();
             uint32_t seen = 0;
-            for (int i = 0; i < wave; ++i) seen += S.wave_u32[i];
-            walk([&](int g, bool q, const float *x) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) seen += i < wave ? S.wave_u32[i] : 0;
+            walk(need, [&](int g, const float *x) {
                 uint32_t c = 0;
                 if (tau > KEY_NONE)
 #pragma unroll
@@ -845,11 +994,12 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
                 }
                 w = sum16(w);
                 const uint32_t first = (uint32_t)__shfl((int)rank0, lane & 48, 64);
-                if (q && (lane & 15) == 15) {
+                if (g >= 0 && (lane & 15) == 15) {
                     mass[g] = w;
                     top[g] = first;
                 }
                 seen += lane_of(upto, 63);
+                return true;
             });
         }
         __syncthreads();
@@ -948,7 +1098,10 @@ template <int XD> int launch(const SampleArgs &A, void *workspace, hipStream_t s
             B.action = A.action + r;
             const double *row_mass = mass + r * groups;
             const uint32_t *row_top = top + r * groups;
-            hipLaunchKernelGGL((k_sample_groups<XD>), dim3((A.v + 2047) / 2048, (unsigned)B.n), dim3(256), 0, s, B, groups, (double *)row_mass, (uint32_t *)row_top);
+            // four tiles a workgroup share its settings; not where that leaves CUs without one
+            const bool many = B.n * ((A.v + 8191) / 8192) >= 1024;
+            if (many) hipLaunchKernelGGL((k_sample_groups<XD, 4>), dim3((A.v + 8191) / 8192, (unsigned)B.n), dim3(256), 0, s, B, groups, (double *)row_mass, (uint32_t *)row_top);
+            else hipLaunchKernelGGL((k_sample_groups<XD, 1>), dim3((A.v + 2047) / 2048, (unsigned)B.n), dim3(256), 0, s, B, groups, (double *)row_mass, (uint32_t *)row_top);
             MZ_LAUNCH_CHECK("k_sample_groups");
             // up to a row per CU: sixteen waves each; more rows: eight waves each, so that a CU works on two
             if (A.n <= 256) hipLaunchKernelGGL((k_sample_row<XD, 16, 8>), dim3((unsigned)B.n), dim3(1024), (size_t)groups * 12, s, B, groups, row_mass, row_top);
@@ -999,6 +1152,7 @@ extern "C" int mz_sample_actions(const mz_sample_args *a, void *workspace, int64
     A.min_p_of = a->min_p_of;
     A.action = a->action;
     A.temperature = a->temperature;
+    A.c = a->temperature > 0.0 ? 1.4426950408889634 / a->temperature : 0.0;
     A.top_p = a->top_p;
     A.min_p = a->min_p;
     A.top_k = (int)std::min<int64_t>(a->top_k, a->v);

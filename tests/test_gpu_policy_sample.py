@@ -65,7 +65,7 @@ def _check(x, u, **kw):
 
 SETTINGS = [dict(), dict(temperature=0.0), dict(temperature=0.25), dict(top_k=1), dict(top_k=5), dict(top_p=0.9), dict(top_p=0.3, temperature=1.7), dict(min_p=0.05),
             dict(top_k=40, top_p=0.8, temperature=0.7), dict(top_k=300, top_p=0.95, min_p=0.01), dict(top_p=0.97, min_p=0.2), dict(top_p=0.0), dict(min_p=1.0),
-            dict(top_k=10 ** 9, top_p=0.999), dict(top_k=2500, top_p=0.5, temperature=2.0), dict(top_p=0.999999, temperature=3.0)]
+            dict(top_k=10 ** 9, top_p=0.999), dict(top_k=2500, top_p=0.5, temperature=2.0), dict(top_k=15000, top_p=0.99, temperature=3.0), dict(min_p=1e-4, temperature=2.0), dict(top_p=0.999999, temperature=3.0)]
 SHAPES = [(1, 1), (5, 2), (3, 63), (9, 64), (64, 65), (5, 128), (5, 129), (7, 500), (4, 512), (5, 513), (3, 1000), (6, 2047), (3, 2048), (3, 2049), (4, 4096), (3, 4097), (5, 5003), (2, 8192), (3, 8193), (3, 32768), (2, 100003), (2, 131072)]
 
 
