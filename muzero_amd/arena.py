@@ -15,6 +15,7 @@ import torch
 from . import _lib as L
 from . import config
 from .env import DT, BatchedEnv
+from .policy import sample_actions
 from .selfplay import SelfPlayEngine
 
 NUM_SIMULATIONS = 100   # test.py:143
@@ -47,6 +48,8 @@ def play_games(black_net, white_net, n_games, num_simulations=NUM_SIMULATIONS, t
                device="cuda", use_graph=True, seed=1261, engines=None):
     """n_games lock-step games, `black_net` moving for BLACK and `white_net` for WHITE (the loop of
     test.py:45-65).  Networks follow the engine protocol (InferenceEngine / NetworkAdapter).
+    num_simulations=0: no search, every move straight from the mover's policy over its legal moves (policy.sample_actions at the same
+    temperature) -- what the networks know without the tree.
     u: optional (steps, n) float64 uniforms for the sampled moves.  Returns ArenaResult with actions
     (steps, n) uint8 and the final disc counts (test.py:67-68)."""
     n, T = int(n_games), int(max_steps if max_steps is not None else config.max_moves)
@@ -54,7 +57,7 @@ def play_games(black_net, white_net, n_games, num_simulations=NUM_SIMULATIONS, t
     if engines is None:
         engines = {}
     for net in (black_net, white_net):
-        if id(net) not in engines:
+        if num_simulations and id(net) not in engines:
             engines[id(net)] = SelfPlayEngine(n, net, num_simulations=num_simulations, device=dev, use_graph=use_graph, seed=seed)
     env = BatchedEnv(n, dev)
     hw = torch.zeros((T + 1, n), dtype=torch.int64, device=dev)
@@ -65,12 +68,17 @@ def play_games(black_net, white_net, n_games, num_simulations=NUM_SIMULATIONS, t
     gen.manual_seed(seed)
     bad = torch.zeros(n, dtype=torch.bool, device=dev)
     for t in range(T):
-        eng = engines[id(black_net if t % 2 == 0 else white_net)]  # BLACK moves on even steps (reversi.py:54,137,176)
-        image = controller_image(hw, hb, t, n, eng.dtype)
-        eng.env = env
-        visits, _ = eng.search(image, noise=None)   # expand_node + run_mcts, no add_exploration_noise (test.py:37-41)
+        net = black_net if t % 2 == 0 else white_net  # BLACK moves on even steps (reversi.py:54,137,176)
         ut = u[t].contiguous() if u is not None else torch.rand(n, dtype=torch.float64, device=dev, generator=gen)
-        a = softmax_sample(visits, temperature, ut)
+        if num_simulations:
+            eng = engines[id(net)]
+            image = controller_image(hw, hb, t, n, eng.dtype)
+            eng.env = env
+            visits, _ = eng.search(image, noise=None)   # expand_node + run_mcts, no add_exploration_noise (test.py:37-41)
+            a = softmax_sample(visits, temperature, ut)
+        else:
+            probs = net.initial(controller_image(hw, hb, t, n, getattr(net, "dtype", torch.float32)))[1]
+            a = sample_actions(probs.float().log(), ut, temperature, legal=env.legal).to(torch.uint8)   # -1 (a policy without mass) is refused as a move
         _, status = env.step(a)   # finished games report MZ_ST_DONE and stay untouched
         bad |= status == L.ST_ILLEGAL
         actions[t].copy_(a)

@@ -37,7 +37,8 @@ from . import train as T
 
 class MuZeroLoop:
     def __init__(self, games_per_rank, device="cuda", infer_dtype=torch.bfloat16, num_simulations=None, window_size=None,
-                 batch_size=None, seed=1261, use_graph=True, group=None, replay_mode="replicated", train_convs="fp32", infer_tower="auto"):
+                 batch_size=None, seed=1261, use_graph=True, group=None, replay_mode="replicated", train_convs="fp32", infer_tower="auto",
+                 max_grad_norm=None, policy_from_logits=False):
         """replay_mode "replicated": trajectories are all_gathered and every rank holds the whole window (what
         BASELINE configs[3] describes); "sharded": no gather at all -- every rank keeps only the games it played (1/N of the
         window), all ranks make the same global draws and each trains on the draws that hit its own games, with the
@@ -46,7 +47,8 @@ class MuZeroLoop:
         gradients on the hand-written matrix-core kernels (bf16 operands, fp32 sums and master weights: train.update_weights
         hip_convs); "hip_x3": those kernels in split precision (three bf16 products per fp32 product: close to fp32).
         infer_tower: InferenceEngine's tower ("auto": the bf16 HIP kernel for infer_dtype bf16; "hip_x3" with infer_dtype float32:
-        self-play at the reference's fp32 precision on the split-precision tower kernel)."""
+        self-play at the reference's fp32 precision on the split-precision tower kernel).
+        max_grad_norm, policy_from_logits: train.update_weights' (None, False: the reference's step)."""
         self.group = group
         self.world = dist.get_world_size(group) if T._dist_on(group) else 1
         self.rank = dist.get_rank(group) if self.world > 1 else 0
@@ -71,6 +73,7 @@ class MuZeroLoop:
         if train_convs not in ("fp32", "hip", "hip_x3"):
             raise ValueError("train_convs must be 'fp32', 'hip' or 'hip_x3'")
         self.hip_convs = {"fp32": False, "hip": True, "hip_x3": "x3"}[train_convs]
+        self.train_options = dict(max_grad_norm=max_grad_norm, policy_from_logits=policy_from_logits)
         self.games_per_rank = int(games_per_rank)
         window = int(window_size if window_size is not None else config.window_size)
         if replay_mode == "sharded":
@@ -109,7 +112,7 @@ class MuZeroLoop:
                     if r == self.rank]
             batch = self.replay.sample_batch(K, [li for li, _ in mine], [p for _, p in mine]) if mine else None
             scale = len(mine) * self.world / self.batch_size
-        return T.update_weights(self.optimizer, self.network, batch, self.bucket, self.group, loss_scale=scale, hip_convs=self.hip_convs)
+        return T.update_weights(self.optimizer, self.network, batch, self.bucket, self.group, loss_scale=scale, hip_convs=self.hip_convs, **self.train_options)
 
     def _publish(self):
         self.storage.save_network(self.network.state_dict())

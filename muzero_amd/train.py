@@ -62,6 +62,12 @@ class FlatGradBucket:
         dist.all_reduce(self.flat, op=dist.ReduceOp.SUM, group=group)
         self.flat.div_(dist.get_world_size(group))
 
+    def clip(self, max_norm):
+        """scale all gradients to a 2-norm of at most max_norm (gradnorm.clip_grad_norm on the one buffer: two launches, GPU only);
+        returns the norm they had, a 0-d tensor that is not waited for"""
+        from .gradnorm import clip_grad_norm
+        return clip_grad_norm(self.flat, max_norm)
+
 
 def make_optimizer(network):
     """train_network's optimiser (main.py:206): SGD lr 1e-3, momentum config.momentum and -- a quirk of
@@ -280,9 +286,11 @@ def _dynamics_deferred(dyn, x, dw):
     return torch.relu(dw.conv(h, seq[5]))
 
 
-def muzero_loss_batched(network, batch, dw):
+def muzero_loss_batched(network, batch, dw, policy_from_logits=False):
     """muzero_loss with the heads batched over the unroll and the Dynamics weight gradients deferred into dw
-    (call dw.flush() after backward).  Returns (p_loss, v_loss)."""
+    (call dw.flush() after backward).  Returns (p_loss, v_loss).
+    policy_from_logits: p_loss by policy.cross_entropy on what stands before the policy head's softmax -- the same function, but a
+    probability that underflows to 0 gives a large loss instead of 0 * log 0 = NaN, in two launches forward and one backward."""
     dev = next(network.parameters()).device
     image, actions, target_values, target_policies = (torch.as_tensor(x, dtype=torch.float32).to(dev) for x in batch)
     if dw.hip and image.is_cuda:
@@ -294,6 +302,13 @@ def muzero_loss_batched(network, batch, dw):
         hidden = _dynamics_deferred(network.dynamics, torch.cat((hidden, action), dim=1), dw)
         hiddens.append(hidden)
     K1, B = len(hiddens), image.shape[0]
+    if policy_from_logits:
+        from .policy import cross_entropy
+        h = torch.cat(hiddens)
+        logits = network.prediction.policy_head[:-1](h)               # all but the softmax
+        p_value = network.prediction.value_head(h).view(K1, B)
+        p_loss = cross_entropy(logits, target_policies.reshape(K1 * B, -1))
+        return p_loss, torch.sum((target_values - p_value) ** 2) / B
     p_policy, p_value = network.prediction(torch.cat(hiddens))        # ((K+1) B, 65), ((K+1) B, 1): rows k * B + b
     p_policy = p_policy.view(K1, B, -1)
     p_value = p_value.view(K1, B)
@@ -302,7 +317,8 @@ def muzero_loss_batched(network, batch, dw):
     return p_loss, v_loss
 
 
-def update_weights(optimizer, network, batch, bucket=None, group=None, amp_dtype=None, loss_scale=1.0, batched=None, hip_convs=False):
+def update_weights(optimizer, network, batch, bucket=None, group=None, amp_dtype=None, loss_scale=1.0, batched=None, hip_convs=False,
+                   max_grad_norm=None, policy_from_logits=False):
     """main.py:230-272.  With `bucket` (FlatGradBucket over network.parameters()) the gradients are
     averaged over the ranks of `group` by ONE all-reduce between backward and optimizer.step.
     amp_dtype (e.g. torch.bfloat16): run the forward/backward convolutions under torch.autocast (fp32 master
@@ -315,7 +331,13 @@ def update_weights(optimizer, network, batch, bucket=None, group=None, amp_dtype
     hip_convs: the gradients of the towers' 3x3, 128 -> 128 convolutions through the hand-written matrix-core kernels
     (muzero_amd/convgrad.py: operands rounded to bf16, fp32 sums; fp32 master weights and optimiser) instead of MIOpen's fp32
     kernels; implies batched.  "x3": the same kernels in split precision (every fp32 product as three bf16 MFMA products: close to
-    fp32, tests/test_gpu_train.py holds it to the reference's recorded gradients).  False = the reference's fp32 arithmetic."""
+    fp32, tests/test_gpu_train.py holds it to the reference's recorded gradients).  False = the reference's fp32 arithmetic.
+    max_grad_norm: scale the (averaged) gradients to a 2-norm of at most this before the step (gradnorm.clip_grad_norm); None = the
+    reference's step, which has no such guard.  policy_from_logits: see muzero_loss_batched; implies batched.  Both need the GPU."""
+    if (max_grad_norm is not None or policy_from_logits) and not next(network.parameters()).is_cuda:
+        raise RuntimeError("update_weights(max_grad_norm=, policy_from_logits=) needs the network on a GPU: the kernels have no CPU fallback")
+    if policy_from_logits and amp_dtype is not None:
+        raise ValueError("policy_from_logits goes with the fp32 and the hip_convs forms, not with amp_dtype")
     if bucket is not None:
         bucket.zero()
     else:
@@ -338,8 +360,10 @@ def update_weights(optimizer, network, batch, bucket=None, group=None, amp_dtype
                 if not next(network.parameters()).is_cuda:   # no CPU stand-in for the HIP kernels
                     raise RuntimeError("update_weights(hip_convs=%r) needs the network on a GPU: the hand-written convolution kernels have no CPU fallback" % (hip_convs,))
                 batched = True
+            if policy_from_logits:
+                batched = True
             dw = DeferredWeightGrads(hip=hip_convs if hip_convs else False) if batched else None
-            p_loss, v_loss = muzero_loss_batched(network, batch, dw) if batched else muzero_loss(network, batch)
+            p_loss, v_loss = muzero_loss_batched(network, batch, dw, policy_from_logits) if batched else muzero_loss(network, batch)
         total = p_loss + v_loss
         (total if loss_scale == 1.0 else total * float(loss_scale)).backward()
         if amp_dtype is None and dw is not None:
@@ -348,6 +372,12 @@ def update_weights(optimizer, network, batch, bucket=None, group=None, amp_dtype
         bucket.all_reduce_mean(group)
     elif _dist_on(group):
         raise RuntimeError("data-parallel update_weights needs a FlatGradBucket")
+    if max_grad_norm is not None:      # behind the all-reduce: every rank scales the same gradients by the same factor
+        if bucket is not None:
+            bucket.clip(max_grad_norm)
+        else:
+            from .gradnorm import clip_grad_norm
+            clip_grad_norm([p.grad for p in network.parameters() if p.grad is not None], max_grad_norm)
     optimizer.step()
     if LOG is not None and network.steps % 10 == 0:   # main.py:268-269; the float() is a device sync
         LOG('step {}: p_loss {:.4f} v_loss {:.4f}'.format(network.steps, float(p_loss.detach()), float(v_loss.detach())))
@@ -413,11 +443,12 @@ def load_checkpoint(network, path, optimizer=None):
 
 
 def train_network(network, optimizer, storage, replay_buffer, training_steps=None, device=None, group=None,
-                  checkpoint_dir="./models", sleep=None, on_publish=None):
+                  checkpoint_dir="./models", sleep=None, on_publish=None, max_grad_norm=None, policy_from_logits=False):
     """main.py:201-227: sample a batch, update, publish the weights every config.checkpoint_interval
     steps, save every 1000 steps.  `optimizer` is replaced exactly as the reference does (main.py:206).
     `sleep` defaults to 0 (the reference sleeps config.training_interval = 0.5 s per step to let its CPU
-    actors keep up; pass it to reproduce that pacing).  Returns the list of (p_loss, v_loss)."""
+    actors keep up; pass it to reproduce that pacing).  max_grad_norm, policy_from_logits: see update_weights.
+    Returns the list of (p_loss, v_loss)."""
     network.train()
     if device is not None:
         network.to(device)
@@ -440,7 +471,7 @@ def train_network(network, optimizer, storage, replay_buffer, training_steps=Non
             batch = replay_buffer.sample_batch(config.num_unroll_steps, idx[sl], pos[sl])
         else:
             batch = replay_buffer.sample_batch(config.num_unroll_steps)
-        losses.append(update_weights(optimizer, network, batch, bucket, group))
+        losses.append(update_weights(optimizer, network, batch, bucket, group, max_grad_norm=max_grad_norm, policy_from_logits=policy_from_logits))
         if i % config.checkpoint_interval == 0:
             state_dict = network.state_dict()
             if storage is not None:

@@ -98,3 +98,13 @@ def test_sample_workspace_is_checked():
     with pytest.raises(L.MzError, match="null arguments"):
         L.call("mz_sample_actions", None, 1 << 40, 1 << 30, None)
     L.call("mz_sample_actions", C.byref(_sample(L, n=0, logits=None, u=None, action=None)), None, 0, None)   # no rows: nothing to do
+
+
+def test_training_options_need_the_gpu():
+    from muzero_amd import train as T
+    from muzero_amd.network import Network
+    net = Network()
+    opt = T.make_optimizer(net)
+    for kw in (dict(max_grad_norm=1.0), dict(policy_from_logits=True)):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            T.update_weights(opt, net, None, T.FlatGradBucket(net.parameters()), **kw)
