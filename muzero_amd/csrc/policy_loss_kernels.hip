@@ -8,7 +8,8 @@
 // Bound by memory: x and t are read, the gradient is written.  So the loss and the gradient come out of ONE pass: the row stays in registers between
 // its sums and its gradient (one wave per row up to 512 actions, one workgroup above), and a training step reads x and t once, not twice.  Rows that
 // are too long for a workgroup's registers, and few long rows, are cut into chunks: one launch for the chunks' sums, one that joins them and writes
-// the gradient.  Softmax statistics and row sums are f32, sums over rows 64 bits; 16-bit gradients are rounded once.
+// the gradient (both read x and t: 5 parts of traffic for 3; in slabs of rows that would stay in the last-level cache between the two launches it
+// was slower, 512 x 131072 f32: 310 us in slabs of 96 MB, 263 us without).  Softmax statistics and row sums are f32, sums over rows 64 bits; 16-bit gradients are rounded once.
 #include <math.h>
 #include <algorithm>
 #include "numeric.h"
@@ -318,18 +319,10 @@ __global__ void __launch_bounds__(1024) k_loss_sum(const float *row_loss, int64_
 // ---- host side -------------------------------------------------------------------------------------------------------------------
 constexpr int64_t MAX_V = 1 << 24, MAX_N = (1 << 22) - 1;   // a launch has fewer than 2^32 threads
 
-struct Plan {
-    int chunk, chunks;
-    int64_t slab;          // rows of one pair of launches
-};
-// chunks of 8192 actions or more; a slab's rows are read again by the second launch while the last-level cache (256 MB) still has them
-Plan plan_chunks(int64_t n, int64_t v, int bytes_per) {
-    Plan p;
-    p.chunk = (int)std::max<int64_t>(8192, ((v + CHUNKS - 1) / CHUNKS + 2047) / 2048 * 2048);
-    p.chunks = (int)((v + p.chunk - 1) / p.chunk);
-    p.slab = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(n, 65535), ((int64_t)96 << 20) / (v * bytes_per)));
-    return p;
-}
+constexpr int64_t SLAB = 65535;         // rows of one pair of launches: what a grid's second dimension takes
+// chunks of 8192 actions or more
+int chunk_size(int64_t v) { return (int)std::max<int64_t>(8192, ((v + CHUNKS - 1) / CHUNKS + 2047) / 2048 * 2048); }
+int chunk_count(int64_t v) { return (int)((v + chunk_size(v) - 1) / chunk_size(v)); }
 
 template <int XD, int TD> int launch(const LossArgs &A, Stat *part, hipStream_t s) {
     constexpr int VEC = Elem<XD>::VEC;
@@ -343,13 +336,16 @@ template <int XD, int TD> int launch(const LossArgs &A, Stat *part, hipStream_t 
     else if (!few && vecs <= 256 * 4) hipLaunchKernelGGL((k_loss_row<XD, TD, 256, 4>), dim3(rows), dim3(256), 0, s, A);
     else if (!few && vecs <= 512 * 4) hipLaunchKernelGGL((k_loss_row<XD, TD, 512, 4>), dim3(rows), dim3(512), 0, s, A);
     else if (!few && vecs <= 512 * 8) hipLaunchKernelGGL((k_loss_row<XD, TD, 512, 8>), dim3(rows), dim3(512), 0, s, A);
+    else if (!few && XD == TD && vecs <= 1024 * 8) {   // f32 targets beside 16-bit logits do not fit the registers
+        if constexpr (XD == TD) hipLaunchKernelGGL((k_loss_row<XD, TD, 1024, 8>), dim3(rows), dim3(1024), 0, s, A);
+    }
     else {
-        const Plan p = plan_chunks(A.n, A.v, elem_bytes(XD) + elem_bytes(TD));
-        for (int64_t r = 0; r < A.n; r += p.slab) {
-            const dim3 grid((unsigned)p.chunks, (unsigned)std::min<int64_t>(p.slab, A.n - r));
-            hipLaunchKernelGGL((k_loss_part<XD, TD>), grid, dim3(256), 0, s, A, r, p.chunk, part);
+        const int chunk = chunk_size(A.v);
+        for (int64_t r = 0; r < A.n; r += SLAB) {
+            const dim3 grid((unsigned)chunk_count(A.v), (unsigned)std::min(SLAB, A.n - r));
+            hipLaunchKernelGGL((k_loss_part<XD, TD>), grid, dim3(256), 0, s, A, r, chunk, part);
             MZ_LAUNCH_CHECK("k_loss_part");
-            hipLaunchKernelGGL((k_loss_join<XD, TD>), grid, dim3(256), 0, s, A, r, p.chunk, (const Stat *)part);
+            hipLaunchKernelGGL((k_loss_join<XD, TD>), grid, dim3(256), 0, s, A, r, chunk, (const Stat *)part);
             MZ_LAUNCH_CHECK("k_loss_join");
         }
     }
@@ -361,8 +357,7 @@ template <int XD, int TD> int launch(const LossArgs &A, Stat *part, hipStream_t 
 
 extern "C" int64_t mz_policy_loss_workspace_bytes(int64_t n, int64_t v) {
     if (n < 0 || n > MAX_N || v < 1 || v > MAX_V) return -1;
-    const Plan p = plan_chunks(n, v, 4);        // the smallest bytes per action have the largest slab
-    return std::max<int64_t>(n, 1) * 4 + 16 + p.slab * p.chunks * (int64_t)sizeof(Stat);
+    return std::max<int64_t>(n, 1) * 4 + 16 + std::min(SLAB, n) * chunk_count(v) * (int64_t)sizeof(Stat);
 }
 
 extern "C" int mz_policy_loss(const mz_policy_loss_args *a, void *workspace, int64_t workspace_bytes, void *stream) {
