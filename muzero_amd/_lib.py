@@ -133,8 +133,8 @@ SIGNATURES = {
     "mz_restower_x3_stamps": [_p, _p, _p, _p, _i64, _p, _p],
     "mz_tower_x3_pack_ends": [_p, _i32, _p, _p, _p],
     "mz_tower_x3_forward": [_p, _p, _p, _p, _p, _i32, _p, _p, _i64, _p],
-    "mz_sample_actions": [C.POINTER(SampleArgs), _p, _i64, _p],
-    "mz_policy_loss": [C.POINTER(PolicyLossArgs), _p, _i64, _p],
+    "mz_sample_actions": [_p, _p, _i64, _p],   # SampleArgs, or its bytes
+    "mz_policy_loss": [_p, _p, _i64, _p],      # PolicyLossArgs, or its bytes
     "mz_grad_norm": [_p, _i32, _p, _i64, _p, _p],
     "mz_grad_clip": [_p, _i32, C.c_double, _p, _i64, _p, _p],
     "mz_inference_x3_forward": [_p, _p, _p, _p, _p, _i32, C.POINTER(HeadsWeights), _p, _p, _p, _p, _i64, _p],

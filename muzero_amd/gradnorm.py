@@ -4,12 +4,15 @@ loss.backward() and optimizer.step() (main.py:266-267) when a step must not be a
 A list of tensors is one operator: one launch per 128 tensors for the norm and one for the scaling, whatever their sizes; the flat
 buffer of a ``train.FlatGradBucket`` is a list of one.  Nothing here waits for the GPU.  No CPU fallback: host tensors raise."""
 import array
+import operator
 
 import torch
 
 from . import _lib as L
 
 _DT = {torch.float32: L.MZ_F32, torch.bfloat16: L.MZ_BF16, torch.float16: L.MZ_F16}
+_T = torch.Tensor
+_DTYPE_OF = operator.attrgetter("dtype")
 
 
 def _dense(t):
@@ -25,23 +28,25 @@ def _dense(t):
 
 
 def _columns(who, tensors):
-    """-> pointers, sizes, dtype codes and GPU index of a list that the kernels can take.  (Most of a call's time on the host: one pass over the
-    list that asks every tensor once, and the checks on its columns.)"""
+    """-> pointers, sizes, dtype codes, GPU index of a list that the kernels can take, and whether all are contiguous.  (Most of a call's time on the host: each
+    question goes over the whole list at once, and the checks over the answers.)"""
     if not tensors:
         raise L.MzError("%s: needs at least one tensor" % who)
-    ptrs, sizes, dtypes, gpus, together = zip(*[(t.data_ptr(), t.numel(), t.dtype, t.get_device(), t.is_contiguous()) for t in tensors])
+    gpus = list(map(_T.get_device, tensors))
     index = gpus[0]
     if index < 0 or gpus.count(index) != len(gpus):
         raise L.MzError("%s: muzero_amd kernels need device tensors, all on one GPU; got %s (no CPU fallback)" % (who, sorted({str(t.device) for t in tensors})))
+    dtypes = list(map(_DTYPE_OF, tensors))
     kinds = set(dtypes)
     if not kinds <= _DT.keys():
         raise L.MzError("%s: float32, bfloat16 or float16 tensors, got %s" % (who, kinds - _DT.keys()))
-    if not all(together):
+    together = all(map(_T.is_contiguous, tensors))
+    if not together:
         for t in tensors:
             if not _dense(t):
                 raise L.MzError("%s: the elements of a tensor have to lie together, got shape %s with strides %s" % (who, tuple(t.shape), t.stride()))
     codes = [_DT[dtypes[0]]] * len(dtypes) if len(kinds) == 1 else [_DT[d] for d in dtypes]
-    return ptrs, sizes, codes, index
+    return list(map(_T.data_ptr, tensors)), list(map(_T.numel, tensors)), codes, index, together
 
 
 def _call(name, dev, table_columns, index, *args):
@@ -62,7 +67,7 @@ def grad_norm(tensors):
     elements lying together in any order of the axes) as a 0-d float32 tensor.  The sums are held in 64 bits in a fixed order.
     inf or NaN among the elements gives inf or NaN."""
     tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
-    ptrs, sizes, codes, index = _columns("grad_norm", tensors)
+    ptrs, sizes, codes, index, _ = _columns("grad_norm", tensors)
     return _call("mz_grad_norm", tensors[0].device, (ptrs, ptrs, sizes, codes), index)
 
 
@@ -73,7 +78,7 @@ def clip_grad_norm(tensors, max_norm, out=None):
     factor is 0, with a NaN it is NaN, as the formula has it: the returned norm says so, and the step can be left out."""
     who = "clip_grad_norm"
     tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
-    ptrs, sizes, codes, index = _columns(who, tensors)
+    ptrs, sizes, codes, index, together = _columns(who, tensors)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise L.MzError("%s: max_norm has to be 0 or more, got %r" % (who, max_norm))
@@ -81,12 +86,12 @@ def clip_grad_norm(tensors, max_norm, out=None):
         outs, dst, dst_codes = tensors, ptrs, codes
     else:
         outs = [out] if torch.is_tensor(out) else list(out)
-        dst, _, dst_codes, oindex = _columns(who + " out", outs)
+        dst, _, dst_codes, oindex, out_together = _columns(who + " out", outs)
         if len(outs) != len(tensors) or oindex != index:
             raise L.MzError("%s: out needs one tensor per gradient, on their GPU" % who)
-        for t, o in zip(tensors, outs):
-            if o.shape != t.shape or (not (o.is_contiguous() and t.is_contiguous()) and o.stride() != t.stride()):
-                raise L.MzError("%s: out has to have the gradients' shapes and strides, got %s %s for %s %s" % (who, tuple(o.shape), o.stride(), tuple(t.shape), t.stride()))
+        if [t.shape for t in tensors] != [o.shape for o in outs] or (not (together and out_together) and any(
+                o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous()) for t, o in zip(tensors, outs))):
+            raise L.MzError("%s: out has to have the gradients' shapes and strides" % who)
         if dst_codes != codes and any(d != s and d != L.MZ_F32 for s, d in zip(codes, dst_codes)):
             raise L.MzError("%s: out has the gradients' dtype or float32" % who)
     types = [s | d << 32 for s, d in zip(codes, dst_codes)]

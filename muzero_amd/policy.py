@@ -7,13 +7,16 @@ logarithm of the probabilities, which differs from it by a constant per row).  R
 are actions: this game's 65 or any other number.  ``legal`` says which of them may be played: a bool tensor of the logits' shape, or
 for 65 actions the (n,) int64 bitboards that ``BatchedEnv.legal`` holds (the pass is legal where no square is).  No CPU fallback:
 host tensors raise."""
-import ctypes as C
+import struct
 
 import torch
 
 from . import _lib as L
 
 _DT = {torch.float32: L.MZ_F32, torch.bfloat16: L.MZ_BF16, torch.float16: L.MZ_F16}
+# the argument structures of include/muzero_amd.h as bytes: a third of the time that filling a ctypes.Structure takes
+_LOSS_ARGS = struct.Struct("9Q6qd4i").pack      # mz_policy_loss_args
+_SAMPLE_ARGS = struct.Struct("9Q5q3di4x").pack  # mz_sample_args
 
 
 def _rows(who, name, t, shape=None, dtypes=tuple(_DT)):
@@ -39,16 +42,16 @@ def _per_row(who, name, t, n, dtype, dev):
 
 
 def _legal(who, legal, logits):
-    """-> (pointer of the bytes, their row stride, pointer of the bitboards)"""
+    """-> (pointer of the bytes, their row stride, pointer of the bitboards); 0: none"""
     if legal is None:
-        return None, 0, None
+        return 0, 0, 0
     if legal.device != logits.device:
         raise L.MzError("%s: legal has to be on the logits' device, got %s (no CPU fallback)" % (who, legal.device))
     if legal.dtype == torch.int64:
         if logits.shape[1] != 65:
             raise L.MzError("%s: bitboards go with 65 actions, the logits have %d" % (who, logits.shape[1]))
-        return None, 0, _per_row(who, "legal", legal, logits.shape[0], torch.int64, logits.device)
-    return legal.data_ptr(), _rows(who, "legal", legal, logits.shape, (torch.bool,)), None
+        return 0, 0, _per_row(who, "legal", legal, logits.shape[0], torch.int64, logits.device)
+    return legal.data_ptr(), _rows(who, "legal", legal, logits.shape, (torch.bool,)), 0
 
 
 class _CrossEntropy(torch.autograd.Function):
@@ -57,29 +60,27 @@ class _CrossEntropy(torch.autograd.Function):
     computes the rows again, so a scaled 16-bit gradient is rounded once, after the scale."""
 
     @staticmethod
-    def forward(ctx, logits, targets, weight, legal, reduction, args):
-        n = args.n
+    def forward(ctx, logits, targets, weight, legal, reduction, head, tail):
+        n, v = logits.shape
         dev = logits.device
         need = ctx.needs_input_grad[0]
         out = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32, device=dev)
+        nbytes = L.lib.mz_policy_loss_workspace_bytes(n, v)
+        if nbytes < 0:
+            raise L.MzError("cross_entropy: (n, actions) = (%d, %d) is too large" % (n, v))
+        grad = None
         if need:
             ctx.save_for_backward(logits, targets, weight, legal)
-        ctx.args = args
-        ctx.ready = None
-        if reduction == "none":
-            args.row_loss = out.data_ptr()
-        else:
-            args.loss = out.data_ptr()
-            if need:
-                ctx.ready = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-                args.grad = ctx.ready.data_ptr()
-        nbytes = L.lib.mz_policy_loss_workspace_bytes(n, args.v)
-        if nbytes < 0:
-            raise L.MzError("cross_entropy: (n, actions) = (%d, %d) is too large" % (n, args.v))
+            ctx.call = head, tail, nbytes
+            if reduction != "none":
+                grad = torch.empty((n, v), dtype=logits.dtype, device=dev)
+            ctx.ready = grad
         if n == 0:
             return out.fill_(float("nan") if reduction == "mean" else 0.0)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        L.call_on(dev.index, "mz_policy_loss", C.byref(args), ws.data_ptr(), nbytes)
+        to = out.data_ptr()
+        rows, loss = (to, 0) if reduction == "none" else (0, to)
+        L.call_on(dev.index, "mz_policy_loss", _LOSS_ARGS(*head, 0, rows, loss, 0 if grad is None else grad.data_ptr(), *tail, 0, 0), ws.data_ptr(), nbytes)
         return out
 
     @staticmethod
@@ -87,19 +88,18 @@ class _CrossEntropy(torch.autograd.Function):
         if torch.is_grad_enabled():            # create_graph: a second derivative is refused when it is asked for
             return _backward_once(ctx, go)
         logits = ctx.saved_tensors[0]          # also says if one of them was changed in place
-        args, grad = ctx.args, ctx.ready
+        grad = ctx.ready
         ctx.ready = None                       # handed out once; a second backward pass gets memory of its own
-        args.skip_one = grad is not None
+        skip = grad is not None
         if grad is None:
             grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        if args.n:
-            go = go.contiguous()
-            args.grad, args.grad_out, args.grad_out_stride = grad.data_ptr(), go.data_ptr(), go.dim()
-            args.row_loss = args.loss = None
-            nbytes = L.lib.mz_policy_loss_workspace_bytes(args.n, args.v)
+        if logits.shape[0]:
+            head, tail, nbytes = ctx.call
+            if not go.is_contiguous():
+                go = go.contiguous()
             ws = torch.empty(nbytes, dtype=torch.uint8, device=grad.device)   # not the forward's: a captured backward keeps its own
-            L.call_on(grad.get_device(), "mz_policy_loss", C.byref(args), ws.data_ptr(), nbytes)
-        return grad, None, None, None, None, None
+            L.call_on(grad.get_device(), "mz_policy_loss", _LOSS_ARGS(*head, go.data_ptr(), 0, 0, grad.data_ptr(), *tail, go.dim(), skip), ws.data_ptr(), nbytes)
+        return grad, None, None, None, None, None, None
 
 
 @torch.autograd.function.once_differentiable
@@ -124,22 +124,22 @@ def cross_entropy(logits, targets, weight=None, legal=None, reduction="mean"):
     if targets.requires_grad or (weight is not None and weight.requires_grad):
         raise L.MzError("%s: targets and weights carry no gradient (detach them)" % who)
     n, v = logits.shape
-    weight_ptr = None if weight is None else _per_row(who, "weight", weight, n, torch.float32, logits.device)
+    weight_ptr = 0 if weight is None else _per_row(who, "weight", weight, n, torch.float32, logits.device)
     allowed, allowed_stride, board = _legal(who, legal, logits)
     if reduction not in ("mean", "sum", "none"):
         raise L.MzError("%s: reduction is 'mean', 'sum' or 'none', got %r" % (who, reduction))
-    args = L.PolicyLossArgs(logits.data_ptr(), targets.data_ptr(), allowed, board, weight_ptr, None, None, None, None, n, v, stride, targets_stride, allowed_stride, v,
-                            1.0 / n if reduction == "mean" and n else 1.0, _DT[dtype], _DT[targets.dtype], 0, 0)
-    return _CrossEntropy.apply(logits, targets, weight, legal, reduction, args)
+    head = logits.data_ptr(), targets.data_ptr(), allowed, board, weight_ptr
+    tail = n, v, stride, targets_stride, allowed_stride, v, 1.0 / n if reduction == "mean" and n else 1.0, _DT[dtype], _DT[targets.dtype]
+    return _CrossEntropy.apply(logits, targets, weight, legal, reduction, head, tail)
 
 
-def _setting(who, name, value, n, dtype, dev, ok):
-    """-> (pointer of one value per row, the one value of all rows)"""
-    if torch.is_tensor(value):
+def _setting(who, name, value, n, dtype, dev, low, high):
+    """-> (pointer of one value per row or 0, the one value of all rows)"""
+    if isinstance(value, torch.Tensor):
         return _per_row(who, name, value, n, dtype, dev), 0
-    if not ok(value):
+    if not low <= value <= high:
         raise L.MzError("%s: %s = %r is out of its range" % (who, name, value))
-    return None, value
+    return 0, value
 
 
 def sample_actions(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, legal=None, out=None):
@@ -159,10 +159,12 @@ def sample_actions(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, le
     n, v = logits.shape
     dev = logits.device
     allowed, allowed_stride, board = _legal(who, legal, logits)
-    temperature_of, temperature = _setting(who, "temperature", temperature, n, torch.float32, dev, lambda x: x == 0 or 1e-30 <= x <= 1e30)
-    top_k_of, top_k = _setting(who, "top_k", top_k, n, torch.int32, dev, lambda x: x == int(x) and 0 <= x < 1 << 62)
-    top_p_of, top_p = _setting(who, "top_p", top_p, n, torch.float32, dev, lambda x: 0 <= x <= 1)
-    min_p_of, min_p = _setting(who, "min_p", min_p, n, torch.float32, dev, lambda x: 0 <= x <= 1)
+    temperature_of, temperature = _setting(who, "temperature", temperature, n, torch.float32, dev, 0.0, 1e30)
+    top_k_of, top_k = _setting(who, "top_k", top_k, n, torch.int32, dev, 0, 1 << 62)
+    top_p_of, top_p = _setting(who, "top_p", top_p, n, torch.float32, dev, 0.0, 1.0)
+    min_p_of, min_p = _setting(who, "min_p", min_p, n, torch.float32, dev, 0.0, 1.0)
+    if int(top_k) != top_k:
+        raise L.MzError("%s: top_k = %r is no whole number" % (who, top_k))
     u_ptr = _per_row(who, "u", u, n, torch.float64, dev)
     nbytes = L.lib.mz_sample_actions_workspace_bytes(n, v)
     if nbytes < 0:
@@ -172,7 +174,7 @@ def sample_actions(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, le
     else:
         _per_row(who, "out", out, n, torch.int32, dev)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    a = L.SampleArgs(logits.data_ptr(), allowed, board, u_ptr, temperature_of, top_k_of, top_p_of, min_p_of, out.data_ptr(), n, v, stride, allowed_stride,
-                     int(top_k), float(temperature), float(top_p), float(min_p), _DT[logits.dtype])
-    L.call_on(dev.index, "mz_sample_actions", C.byref(a), None if ws is None else ws.data_ptr(), nbytes)
+    args = _SAMPLE_ARGS(logits.data_ptr(), allowed, board, u_ptr, temperature_of, top_k_of, top_p_of, min_p_of, out.data_ptr(), n, v, stride, allowed_stride, int(top_k),
+                        temperature, top_p, min_p, _DT[logits.dtype])
+    L.call_on(dev.index, "mz_sample_actions", args, None if ws is None else ws.data_ptr(), nbytes)
     return out

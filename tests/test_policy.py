@@ -108,3 +108,16 @@ def test_training_options_need_the_gpu():
     for kw in (dict(max_grad_norm=1.0), dict(policy_from_logits=True)):
         with pytest.raises(RuntimeError, match="no CPU fallback"):
             T.update_weights(opt, net, None, T.FlatGradBucket(net.parameters()), **kw)
+
+
+def test_argument_structures_as_bytes():
+    """policy.py packs the structures of include/muzero_amd.h itself: the same sizes and places as the ctypes ones"""
+    from muzero_amd import _lib as L
+    from muzero_amd import policy
+    for pack, cls in ((policy._LOSS_ARGS, L.PolicyLossArgs), (policy._SAMPLE_ARGS, L.SampleArgs)):
+        names = [f[0] for f in cls._fields_]
+        values = [1.0 + k if t is C.c_double else k + 1 for k, (_, t) in enumerate(cls._fields_)]
+        raw = pack(*values)
+        assert len(raw) == C.sizeof(cls)
+        a = cls.from_buffer_copy(raw)
+        assert [getattr(a, k) for k in names] == values
