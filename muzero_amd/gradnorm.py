@@ -95,4 +95,6 @@ def clip_grad_norm(tensors, max_norm, out=None):
         if dst_codes != codes and any(d != s and d != L.MZ_F32 for s, d in zip(codes, dst_codes)):
             raise L.MzError("%s: out has the gradients' dtype or float32" % who)
     types = [s | d << 32 for s, d in zip(codes, dst_codes)]
-    return _call("mz_grad_clip", tensors[0].device, (ptrs, dst, sizes, types), index, max_norm)
+    norm = _call("mz_grad_clip", tensors[0].device, (ptrs, dst, sizes, types), index, max_norm)
+    torch.autograd.graph.increment_version(outs)      # autograd's check of tensors changed in place sees these too
+    return norm

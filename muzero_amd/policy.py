@@ -85,8 +85,10 @@ class _CrossEntropy(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, go):
-        if torch.is_grad_enabled():            # create_graph: a second derivative is refused when it is asked for
-            return _backward_once(ctx, go)
+        if torch.is_grad_enabled():            # create_graph: the gradient, and an error when its own is asked for
+            with torch.no_grad():
+                grad = _CrossEntropy.backward(ctx, go)[0]
+            return _NoSecondDerivative.apply(grad.detach().requires_grad_()), None, None, None, None, None, None
         logits = ctx.saved_tensors[0]          # also says if one of them was changed in place
         grad = ctx.ready
         ctx.ready = None                       # handed out once; a second backward pass gets memory of its own
@@ -102,14 +104,19 @@ class _CrossEntropy(torch.autograd.Function):
         return grad, None, None, None, None, None, None
 
 
-@torch.autograd.function.once_differentiable
-def _backward_once(ctx, go):
-    return _CrossEntropy.backward(ctx, go)
+class _NoSecondDerivative(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, grad):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, go):
+        raise L.MzError("cross_entropy: there is no second derivative")
 
 
 def cross_entropy(logits, targets, weight=None, legal=None, reduction="mean"):
     """-sum over the legal actions of targets * log softmax(logits), per row times `weight`: the mean over the n rows, their "sum", or
-    "none" = the (n,) rows, in float32, differentiable in the logits.
+    "none" = the (n,) rows, in float32, differentiable in the logits (once).
 
     logits (n, v) float32 / bfloat16 / float16; targets (n, v) of the same dtype or float32, any non-negative shares (they need not add
     up to 1); rows may be strided, a row's elements lie together.  weight float32 (n,): a row of weight 0 (padding) counts in the mean's n
@@ -177,4 +184,5 @@ def sample_actions(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, le
     args = _SAMPLE_ARGS(logits.data_ptr(), allowed, board, u_ptr, temperature_of, top_k_of, top_p_of, min_p_of, out.data_ptr(), n, v, stride, allowed_stride, int(top_k),
                         temperature, top_p, min_p, _DT[logits.dtype])
     L.call_on(dev.index, "mz_sample_actions", args, None if ws is None else ws.data_ptr(), nbytes)
+    torch.autograd.graph.increment_version(out)
     return out

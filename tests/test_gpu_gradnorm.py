@@ -147,6 +147,16 @@ def test_two_streams_at_once_and_replayed_graphs():
             assert torch.equal(n, grad_norm(x))
 
 
+def test_autograd_notices_what_was_scaled():
+    from muzero_amd.gradnorm import clip_grad_norm
+    x = torch.ones(64, device="cuda", requires_grad=True)
+    y = x * 2.0
+    z = (y * y).sum()                                    # keeps y
+    clip_grad_norm(y, 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+
+
 def test_refusals():
     from muzero_amd import _lib as L
     from muzero_amd.gradnorm import clip_grad_norm, grad_norm

@@ -226,6 +226,32 @@ def test_changed_logits_are_noticed():
         loss.backward()
 
 
+@pytest.mark.parametrize("v", [65, 5000, 70001])
+def test_rows_that_share_their_memory(v):
+    """one row of logits and one mask for all: their gradients add up"""
+    from muzero_amd.policy import cross_entropy
+    n = 5
+    x, t, w, _ = _inputs(n, v, F32, F32, "none", 0, True, seed=v)
+    one = x.detach()[:1].clone().requires_grad_()
+    mask = (torch.rand(1, v, device="cuda") < 0.5).expand(n, v)
+    rows, grad, rtol, gtol, _ = _reference(one.detach().expand(n, v), t, w, mask)
+    loss = cross_entropy(one.expand(n, v), t, weight=w, legal=mask, reduction="sum")
+    assert abs(loss.double().item() - rows.sum().item()) <= rtol.sum().item() + U * abs(rows.sum().item()) + 1e-40
+    got, = torch.autograd.grad(loss, one)
+    tol = gtol.sum(0) + (4 + n) * U * grad.abs().sum(0) + TINY[F32]
+    assert bool(((got[0].double() - grad.sum(0)).abs() <= tol).all())
+
+
+def test_a_second_derivative_is_refused():
+    from muzero_amd.policy import cross_entropy
+    x, t, _, _ = _inputs(4, 65, F32, F32, "none", 0, False, seed=3)
+    want, = torch.autograd.grad(cross_entropy(x, t), x)
+    got, = torch.autograd.grad(cross_entropy(x, t), x, create_graph=True)
+    assert torch.equal(got, want)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        (got.square().sum() + x.sum()).backward()
+
+
 def test_no_rows():
     from muzero_amd.policy import cross_entropy
     x = torch.zeros(0, 65, device="cuda", requires_grad=True)
