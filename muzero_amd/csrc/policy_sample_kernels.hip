@@ -307,25 +307,32 @@ template <int XD, int E> __global__ void __launch_bounds__(256) k_sample_wave(Sa
 // eight actions of a row as they lie there (so that their loads can be under way while others are worked on)
 template <int XD> struct Eight {
     Words<XD, 8> words;
-    uint64_t ok;                                 // a byte each; 0: behind the row's end or not legal, -inf
+    uint64_t ok;                                 // with a mask: a byte each, 0 = not legal
+    __device__ __forceinline__ void none() {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) words.set(j, (typename Elem<XD>::T)(XD == MZ_F32 ? 0xFF800000u : XD == MZ_BF16 ? 0xFF80u : 0xFC00u));
+        ok = ~0ull;
+    }
     __device__ __forceinline__ void load(const SampleArgs &A, int64_t xo, int64_t ao, int at) {
         if (at + 8 <= A.v) {
             words = load_words<XD, 8>(A.x, xo + at);
-            ok = A.allowed ? load_flags(A.allowed, ao + at) : ~0ull;
-        } else {
-            words = {};
-            ok = 0;
+            if (A.allowed) ok = load_flags(A.allowed, ao + at);
+        } else {                                 // behind the row's end: -inf
+            none();
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (at + j < A.v && (!A.allowed || A.allowed[ao + at + j])) {
+                if (at + j < A.v) {
                     words.set(j, ((const MZ_GLOBAL typename Elem<XD>::T *)A.x)[xo + at + j]);
-                    ok |= 0xFFull << j * 8;
+                    if (A.allowed && !A.allowed[ao + at + j]) ok &= ~(0xFFull << j * 8);
                 }
         }
     }
-    __device__ __forceinline__ void unpack(float *x) const {
+    __device__ __forceinline__ void unpack(const SampleArgs &A, float *x) const {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = (ok >> j * 8) & 0xFF ? words.get(j) : -INFINITY;
+        for (int j = 0; j < 8; ++j) x[j] = words.get(j);
+        if (A.allowed)                           // the same for the whole launch
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = (ok >> j * 8) & 0xFF ? x[j] : -INFINITY;
     }
 };
 
@@ -608,7 +615,7 @@ template <int XD, int W> __global__ void __launch_bounds__(64 * W) k_sample_bloc
     float x[8];
     Eight<XD> e;
     e.load(A, row * A.x_stride, row * A.allowed_stride, threadIdx.x * 8);
-    e.unpack(x);
+    e.unpack(A, x);
     uint32_t best = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) best = max(best, x[j] != x[j] ? 0xFFFFFFFFu : key_of(x[j]));
@@ -653,12 +660,12 @@ template <int XD, int TILES> __global__ void __launch_bounds__(256) k_sample_gro
         const int at = first + t * 2048, g = at / GROUP;
         if (t + 1 < TILES) e2.load(A, xo, ao, at + 2048);
         float x[8], m = -INFINITY;
-        e.unpack(x);
+        e.unpack(A, x);
         bool nan = false;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            m = fmaxf(m, x[j]);
-            nan |= x[j] != x[j];
+        for (int j = 0; j < 8; j += 2) {
+            m = fmaxf(m, fmaxf(x[j], x[j + 1]));
+            nan |= __builtin_isunordered(x[j], x[j + 1]);
         }
         const uint32_t key = lane_last16(max16(nan ? 0xFFFFFFFFu : key_of(m)));
         const bool writes = (threadIdx.x & 15) == 15 && g < groups;
@@ -810,16 +817,13 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
                                 if (lane >> 4 == i) mine[d] = g0 + bit;
                             }
                         if (mine[d] >= 0) e[d].load(A, xo, ao, mine[d] * GROUP + (lane & 15) * 8);
-                        else {
-                            e[d].words = {};
-                            e[d].ok = 0;
-                        }
+                        else e[d].none();
                     }
 #pragma unroll
                     for (int d = 0; d < DEPTH; ++d) {
                         if (!__ballot(mine[d] >= 0)) return;
                         float x[8];
-                        e[d].unpack(x);
+                        e[d].unpack(A, x);
                         if (!take(mine[d], x)) return;
                     }
                 }
