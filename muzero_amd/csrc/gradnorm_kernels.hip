@@ -3,7 +3,7 @@
 //   norm = sqrt(sum over tensors and elements of g^2),   dst = src * min(1, max_norm / (norm + 1e-6))
 //
 // Both passes are bound by memory.  The tensors are cut into chunks of equal bytes and a fixed number of workgroups walks over them, so a list of
-// forty ragged tensors costs what one flat buffer of their size does: one launch per 128 tensors and pass.  The list travels in the kernel's
+// forty ragged tensors costs what one flat buffer of their size does: one launch per 256 tensors for the norm, per 128 for the scaling.  The list travels in the kernel's
 // arguments (no copy to the device, so a call can be captured).  Squares and sums are held in 64 bits: no overflow above 1.8e19, no underflow below
 // 1e-23, and the order of the sums is fixed by the chunks, so the norm has the same bits on every call.
 #include <stdlib.h>
@@ -15,37 +15,52 @@ namespace {
 
 using namespace mz;
 
-constexpr int LIST = 128;      // tensors per launch: with their pointers, sizes and types 3.7 KB of the 4 KB that a launch's arguments may take
 constexpr int GRID = 1024;     // workgroups of 256 threads: four per CU
 
-struct GradList {
+// Tensors of one launch: as many as fit the 4 KB that a launch's arguments may take.  A tensor is its pointers, its first chunk and, in 16 bits, the
+// size of its last chunk less one (at most 2^14 - 1) and its type.
+template <bool DST> struct GradList {
+    static constexpr int LIST = DST ? 128 : 256;
     const void *src[LIST];
-    void *dst[LIST];
-    int64_t n[LIST];
+    const void *dst[DST ? LIST : 1];
     uint32_t start[LIST];      // first chunk of each tensor; above the last one 0xFFFFFFFF
-    uint8_t src_dt[LIST], dst_dt[LIST];
+    uint16_t last[LIST];       // (size of the last chunk - 1) | dtype << 14
+    uint8_t dst_dt[DST ? LIST : 1];
     uint32_t chunks;
 };
-static_assert(sizeof(GradList) + 64 <= 4096, "the list has to fit a launch's arguments");
+static_assert(sizeof(GradList<false>) + 64 <= 4096 && sizeof(GradList<true>) + 64 <= 4096, "the list has to fit a launch's arguments");
 
-// the tensor that chunk c belongs to: the last one that starts at or before it
-__device__ __forceinline__ int tensor_of(const GradList &L, uint32_t c) {
-    const int lane = threadIdx.x & 63;
-    const int k = __popcll(__ballot(L.start[lane] <= c)) + __popcll(__ballot(L.start[lane + 64] <= c));
-    return __builtin_amdgcn_readfirstlane(k - 1);
-}
+// chunk c of the list: its tensor (the last one that starts at or before it), its first element, and how many there are
+template <int U, bool DST> struct Chunk {
+    int i, dt;
+    int64_t at;
+    int left;
+    __device__ __forceinline__ Chunk(const GradList<DST> &L, uint32_t c) {
+        const int lane = threadIdx.x & 63;
+        int k = 0;
+#pragma unroll
+        for (int j = 0; j < GradList<DST>::LIST; j += 64) k += (int)__popcll(__ballot(L.start[j + lane] <= c));
+        i = __builtin_amdgcn_readfirstlane(k - 1);
+        const uint32_t end = i + 1 < GradList<DST>::LIST ? min(L.start[i + 1], L.chunks) : L.chunks;
+        const uint32_t last = L.last[i];
+        dt = (int)(last >> 14);
+        const int full = U * 256 * (dt == MZ_F32 ? 4 : 8);
+        at = (int64_t)(c - L.start[i]) * full;
+        left = c + 1 == end ? (int)(last & 0x3FFF) + 1 : full;
+    }
+};
 
 // U vectors of 16 bytes per lane; a tensor's last chunk keeps whole vectors too, so that all of its loads are in flight together, and one element a
 // lane behind them
-template <int DT, int U> __device__ __forceinline__ double square_sum(const void *src, int64_t at, int64_t left) {
+template <int DT, int U> __device__ __forceinline__ double square_sum(const void *src, int64_t at, int left) {
     constexpr int VEC = Elem<DT>::VEC;
     double acc = 0.0;
     Words<DT, VEC> p[U];
-    if (left >= (int64_t)U * 256 * VEC) {
+    if (left == U * 256 * VEC) {
 #pragma unroll
-        for (int k = 0; k < U; ++k) p[k] = load_words<DT, VEC>(src, at + ((int64_t)k * 256 + threadIdx.x) * VEC);
+        for (int k = 0; k < U; ++k) p[k] = load_words<DT, VEC>(src, at + (k * 256 + (int)threadIdx.x) * VEC);
     } else {
-        const int whole = (int)(left / VEC), rest = (int)(left % VEC);
+        const int whole = left / VEC, rest = left % VEC;
 #pragma unroll
         for (int k = 0; k < U; ++k) {
             const int v = k * 256 + threadIdx.x;
@@ -65,16 +80,14 @@ template <int DT, int U> __device__ __forceinline__ double square_sum(const void
     return acc;
 }
 
-template <int U> __global__ void __launch_bounds__(256) k_norm_partial(GradList L, double *partial) {
+template <int U> __global__ void __launch_bounds__(256) k_norm_partial(GradList<false> L, double *partial) {
     __shared__ double red[4];
     double acc = 0.0;
     for (uint32_t c = blockIdx.x; c < L.chunks; c += gridDim.x) {
-        const int i = tensor_of(L, c);
-        const int dt = L.src_dt[i];
-        const int64_t at = (int64_t)(c - L.start[i]) * (U * 256 * (dt == MZ_F32 ? 4 : 8)), left = L.n[i] - at;
-        if (dt == MZ_F32) acc += square_sum<MZ_F32, U>(L.src[i], at, left);
-        else if (dt == MZ_BF16) acc += square_sum<MZ_BF16, U>(L.src[i], at, left);
-        else acc += square_sum<MZ_F16, U>(L.src[i], at, left);
+        const Chunk<U, false> k(L, c);
+        if (k.dt == MZ_F32) acc += square_sum<MZ_F32, U>(L.src[k.i], k.at, k.left);
+        else if (k.dt == MZ_BF16) acc += square_sum<MZ_BF16, U>(L.src[k.i], k.at, k.left);
+        else acc += square_sum<MZ_F16, U>(L.src[k.i], k.at, k.left);
     }
     acc = block_sum<4>(acc, red);
     if (threadIdx.x == 0) partial[blockIdx.x] = acc;
@@ -88,11 +101,11 @@ __global__ void __launch_bounds__(1024) k_norm_final(const double *partial, int 
     if (threadIdx.x == 0) *norm = (float)sqrt(s);
 }
 
-template <int SD, int DD, int U> __device__ __forceinline__ void scale_chunk(const void *src, void *dst, int64_t at, int64_t left, float scale) {
+template <int SD, int DD, int U> __device__ __forceinline__ void scale_chunk(const void *src, void *dst, int64_t at, int left, float scale) {
     constexpr int VEC = Elem<SD>::VEC;
-    const int whole = (int)(min(left, (int64_t)U * 256 * VEC) / VEC);
+    const int whole = left / VEC;
     const int64_t end = at + (int64_t)whole * VEC + threadIdx.x;
-    if (left < (int64_t)U * 256 * VEC && (int)threadIdx.x < (int)(left % VEC)) store_one<DD>(dst, end, load_one<SD>(src, end) * scale);
+    if ((int)threadIdx.x < left % VEC) store_one<DD>(dst, end, load_one<SD>(src, end) * scale);
     Words<SD, VEC> p[U];
 #pragma unroll
     for (int k = 0; k < U; ++k) {
@@ -112,7 +125,7 @@ template <int SD, int DD, int U> __device__ __forceinline__ void scale_chunk(con
 }
 
 // every workgroup adds up the partial sums itself (the same order, so the same norm), which saves a launch between the passes
-template <int U> __global__ void __launch_bounds__(256) k_clip(GradList L, const double *partial, int count, double max_norm, float *norm, int write_norm) {
+template <int U> __global__ void __launch_bounds__(256) k_clip(GradList<true> L, const double *partial, int count, double max_norm, float *norm, int write_norm) {
     __shared__ double red[4];
     double s = 0.0;
     for (int k = threadIdx.x; k < count; k += 256) s += partial[k];
@@ -121,12 +134,12 @@ template <int U> __global__ void __launch_bounds__(256) k_clip(GradList L, const
     const double ratio = max_norm / (s + 1e-6);
     const float scale = ratio >= 1.0 ? 1.0f : (float)ratio;   // a NaN stays one
     for (uint32_t c = blockIdx.x; c < L.chunks; c += gridDim.x) {
-        const int i = tensor_of(L, c);
-        const int sd = L.src_dt[i], dd = L.dst_dt[i];
-        const void *src = L.src[i];
-        void *dst = L.dst[i];
+        const Chunk<U, true> k(L, c);
+        const int sd = k.dt, dd = L.dst_dt[k.i], left = k.left;
+        const int64_t at = k.at;
+        const void *src = L.src[k.i];
+        void *dst = (void *)L.dst[k.i];
         if (scale == 1.0f && src == dst) continue;            // in place and not clipped: the values stay as they are
-        const int64_t at = (int64_t)(c - L.start[i]) * (U * 256 * (sd == MZ_F32 ? 4 : 8)), left = L.n[i] - at;
         if (sd == MZ_F32) scale_chunk<MZ_F32, MZ_F32, U>(src, dst, at, left, scale);
         else if (sd == MZ_BF16) {
             if (dd == MZ_F32) scale_chunk<MZ_BF16, MZ_F32, U>(src, dst, at, left, scale);
@@ -189,28 +202,33 @@ int check_overlap(const char *who, const mz_grad_tensor *t, int32_t count) {
     return MZ_OK;
 }
 
-// the next list of up to LIST non-empty tensors from *i on; returns their count
-int next_list(const mz_grad_tensor *t, int32_t count, int *i, int chunk_bytes, GradList *L) {
+// the next list of non-empty tensors from *i on; returns their count
+template <bool DST> int next_list(const mz_grad_tensor *t, int32_t count, int *i, int chunk_bytes, GradList<DST> *L) {
     int k = 0;
     uint32_t chunks = 0;
-    for (; *i < count && k < LIST; ++*i) {
+    for (; *i < count && k < GradList<DST>::LIST; ++*i) {
         const mz_grad_tensor &x = t[*i];
         if (x.n == 0) continue;
+        const int64_t full = chunk_bytes / elem_bytes(x.src_dtype), parts = (x.n + full - 1) / full;
         L->src[k] = x.src;
-        L->dst[k] = x.dst;
-        L->n[k] = x.n;
+        if (DST) {
+            L->dst[k] = x.dst;
+            L->dst_dt[k] = (uint8_t)x.dst_dtype;
+        }
         L->start[k] = chunks;
-        L->src_dt[k] = (uint8_t)x.src_dtype;
-        L->dst_dt[k] = (uint8_t)x.dst_dtype;
-        chunks += (uint32_t)((x.n * elem_bytes(x.src_dtype) + chunk_bytes - 1) / chunk_bytes);
+        L->last[k] = (uint16_t)((x.n - (parts - 1) * full - 1) | x.src_dtype << 14);
+        chunks += (uint32_t)parts;
         ++k;
     }
     L->chunks = chunks;
-    for (int j = k; j < LIST; ++j) {
+    for (int j = k; j < GradList<DST>::LIST; ++j) {
         L->start[j] = 0xFFFFFFFFu;
-        L->src[j] = L->dst[j] = nullptr;
-        L->n[j] = 0;
-        L->src_dt[j] = L->dst_dt[j] = 0;
+        L->last[j] = 0;
+        L->src[j] = nullptr;
+        if (DST) {
+            L->dst[j] = nullptr;
+            L->dst_dt[j] = 0;
+        }
     }
     return k;
 }
@@ -221,7 +239,7 @@ inline int unroll_for(int64_t bytes) { return bytes < ((int64_t)64 << 20) ? 2 : 
 int partial_sums(const mz_grad_tensor *t, int32_t count, int unroll, double *partial, int *partials, hipStream_t s) {
     *partials = 0;
     for (int i = 0; i < count;) {
-        GradList L;
+        GradList<false> L;
         if (!next_list(t, count, &i, unroll * 4096, &L)) break;
         const int grid = (int)std::min<uint32_t>(L.chunks, GRID);
         if (unroll == 2) hipLaunchKernelGGL((k_norm_partial<2>), dim3(grid), dim3(256), 0, s, L, partial + *partials);
@@ -236,6 +254,7 @@ int partial_sums(const mz_grad_tensor *t, int32_t count, int unroll, double *par
 
 extern "C" int64_t mz_grad_workspace_bytes(int32_t count) {
     if (count < 1) return -1;
+    constexpr int LIST = GradList<false>::LIST;
     return (((int64_t)count + LIST - 1) / LIST) * GRID * (int64_t)sizeof(double);
 }
 
@@ -267,7 +286,7 @@ extern "C" int mz_grad_clip(const mz_grad_tensor *tensors, int32_t count, double
     int partials, first = 1;
     if (int rc = partial_sums(tensors, count, unroll, (double *)workspace, &partials, s)) return rc;
     for (int i = 0; i < count || first;) {
-        GradList L;
+        GradList<true> L;
         if (!next_list(tensors, count, &i, unroll * 4096, &L) && !first) break;   // with nothing but empty tensors the norm is written all the same
         const int grid = (int)std::max<uint32_t>(1, std::min<uint32_t>(L.chunks, GRID));
         if (unroll == 2) hipLaunchKernelGGL((k_clip<2>), dim3(grid), dim3(256), 0, s, L, (const double *)workspace, partials, max_norm, norm, first);

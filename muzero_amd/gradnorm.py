@@ -1,7 +1,7 @@
 """The 2-norm over all gradients of a step and their clipping by it (muzero_amd/csrc/gradnorm_kernels.hip): what stands between
 loss.backward() and optimizer.step() (main.py:266-267) when a step must not be allowed to run away.
 
-A list of tensors is one operator: one launch per 128 tensors for the norm and one for the scaling, whatever their sizes; the flat
+A list of tensors is one operator: one launch per 256 tensors for the norm and per 128 for the scaling, whatever their sizes; the flat
 buffer of a ``train.FlatGradBucket`` is a list of one.  Nothing here waits for the GPU.  No CPU fallback: host tensors raise."""
 import array
 import operator

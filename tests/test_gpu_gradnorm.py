@@ -28,7 +28,7 @@ def _check_clip(outs, ts, want_norm, max_norm):
         assert bool(((o.double() - ref).abs() <= tol).all()), (o.dtype, tuple(t.shape))
 
 
-SIZES = [[1], [2047], [2048], [2049], [65, 1, 128, 147456, 2], [8191, 8193, 16385], [3_000_017], [17_000_003, 5], [7] * 300, [1000 + 37 * i for i in range(131)]]
+SIZES = [[1], [2047], [2048], [2049], [65, 1, 128, 147456, 2], [8191, 8193, 16385], [3_000_017], [17_000_003, 5], [7] * 300, [1000 + 37 * i for i in range(131)], [4095, 4096, 4097] * 100]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])

@@ -36,7 +36,7 @@ def test_lists_are_checked_before_any_launch():
     from muzero_amd import _lib as L
     P = 1 << 40                                  # never read: every call below is refused on the host
     nbytes = L.lib.mz_grad_workspace_bytes(1)
-    assert nbytes > 0 and L.lib.mz_grad_workspace_bytes(129) == 2 * nbytes and L.lib.mz_grad_workspace_bytes(0) == -1
+    assert nbytes > 0 and L.lib.mz_grad_workspace_bytes(257) == 2 * nbytes and L.lib.mz_grad_workspace_bytes(0) == -1
 
     def norm(rows, count=None, ws=P, wb=1 << 20, out=P):
         L.call("mz_grad_norm", _table(L, rows), len(rows) if count is None else count, ws, wb, out, None)
