@@ -690,6 +690,7 @@ template <int W, int N> struct RowShared {
     Shared<W> S;
     float x[W * SEG];
     int32_t index[W * SEG];
+    uint16_t list[MAX_V / GROUP];
 };
 
 template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_sample_row(SampleArgs A, int groups, const double *mass_in, const uint32_t *top_in) {
@@ -785,6 +786,7 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
                         const int step = wave * (16 / W) + i + 1;
                         const double most = ldexp(b, 2 * step) * GROUP;
                         double sum = 0.0;
+#pragma unroll 8
                         for (int g = lane; g < groups; g += 64) sum += fmin(mass[g], most);
                         if (total(sum) < rest) good = step;
                     }
@@ -792,36 +794,48 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
                     low = bound(m + (log2(b) + 2.0 * good) / s.c);
                 }
             }
-            // Every wave owns a run of the groups and walks over those that reach `need`, in order, sixteen lanes to a group, the loads of DEPTH times
-            // four groups under way together; `take` gets a lane's group (-1: none) and its eight actions, and says whether to go on.
-            const int run0 = (int)((int64_t)groups * wave / W), run1 = (int)((int64_t)groups * (wave + 1) / W);
-            auto walk = [&](uint32_t need, auto take) {
+            // the groups that reach `need`, in order, in R.list; their number
+            auto list_groups = [&](uint32_t need) {
+                const int run0 = (int)((int64_t)groups * wave / W), run1 = (int)((int64_t)groups * (wave + 1) / W);
+                int n = 0;
+                for (int g = run0; g < run1; g += 64) n += (int)__popcll(__ballot(g + lane < run1 && top[min(g + lane, groups - 1)] >= need));
+                __syncthreads();
+                if (lane == 0) S.wave_u32[wave] = (uint32_t)n;
+                __syncthreads();
+                int to = 0, all_of_them = 0;
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    const int c = (int)S.wave_u32[i];
+                    to += i < wave ? c : 0;
+                    all_of_them += c;
+                }
+                for (int g = run0; g < run1; g += 64) {
+                    const bool reach = g + lane < run1 && top[min(g + lane, groups - 1)] >= need;
+                    const uint64_t b = __ballot(reach);
+                    if (reach) R.list[to + (int)__popcll(b & lanes_below(lane))] = (uint16_t)(g + lane);
+                    to += (int)__popcll(b);
+                }
+                __syncthreads();
+                return all_of_them;
+            };
+            // Every wave walks over an equal share of the listed groups, in order, sixteen lanes to a group, the loads of DEPTH times four groups under way
+            // together; `take` gets a lane's group (-1: none) and its eight actions, and says whether to go on.
+            auto walk = [&](int listed, auto take) {
                 constexpr int DEPTH = XD == MZ_F32 ? 3 : 4;   // what fits 128 registers
-                int g0 = run0 - 64;
-                uint64_t reach = 0;
-                for (;;) {
+                const int q1 = (int)((int64_t)listed * (wave + 1) / W);
+                for (int q = (int)((int64_t)listed * wave / W); q < q1; q += 4 * DEPTH) {
                     Eight<XD> e[DEPTH];
                     int mine[DEPTH];
 #pragma unroll
                     for (int d = 0; d < DEPTH; ++d) {
-                        while (!reach && g0 + 64 < run1) {
-                            g0 += 64;
-                            reach = __ballot(g0 + lane < run1 && top[min(g0 + lane, groups - 1)] >= need);
-                        }
-                        mine[d] = -1;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (reach) {
-                                const int bit = __ffsll((unsigned long long)reach) - 1;
-                                reach &= reach - 1;
-                                if (lane >> 4 == i) mine[d] = g0 + bit;
-                            }
+                        const int i = q + 4 * d + (lane >> 4);
+                        mine[d] = i < q1 ? (int)R.list[i] : -1;
                         if (mine[d] >= 0) e[d].load(A, xo, ao, mine[d] * GROUP + (lane & 15) * 8);
                         else e[d].none();
                     }
 #pragma unroll
                     for (int d = 0; d < DEPTH; ++d) {
-                        if (!__ballot(mine[d] >= 0)) return;
+                        if (q + 4 * d >= q1) return;
                         float x[8];
                         e[d].unpack(A, x);
                         if (!take(mine[d], x)) return;
@@ -830,19 +844,19 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
             };
             // the actions from `low` on, in their order, each wave's in a segment of its own
             int count = 0;
-            if (bounded)
-                walk(low, [&](int g, const float *x) {
-                    uint32_t c = 0;
+            int listed = list_groups(low);
+            if (bounded) {
+                const float least = value_of(low);
+                walk(listed, [&](int g, const float *x) {
+                    uint32_t n = 0;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (key_of(x[j]) >= low) c |= 1u << j;
-                    if (!__ballot(c)) return true;
-                    const uint32_t n = (uint32_t)__popc(c), upto = scan(n);
+                    for (int j = 0; j < 8; ++j) n += x[j] >= least;
+                    const uint32_t upto = scan(n);
                     int to = count + (int)(upto - n);
                     count += (int)lane_of(upto, 63);
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        if (c >> j & 1) {
+                        if (x[j] >= least) {
                             if (to < SEG) {
                                 R.x[wave * SEG + to] = x[j];
                                 R.index[wave * SEG + to] = g * GROUP + (lane & 15) * 8 + j;
@@ -851,6 +865,8 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
                         }
                     return count <= SEG;
                 });
+            }
+            __syncthreads();
             if (lane == 0) S.wave_u32[wave] = bounded ? (uint32_t)count : SEG + 1u;
             __syncthreads();
             int many = 0, most = 0, start[W + 1];
@@ -904,7 +920,7 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
             if (s.k) {
                 uint32_t t;
                 auto each = [&](auto take) {
-                    walk(low, [&](int, const float *x) {
+                    walk(listed, [&](int, const float *x) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j) take(key_of(x[j]), x[j], [] { return 1ull; });
                         return true;
@@ -925,11 +941,12 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
             }
             if (s.p_on) {
                 const uint32_t lowest = tau > KEY_NONE ? tau : low;
+                listed = list_groups(lowest);
                 double limit;
                 if (massed) limit = s.top_p * all * scale;
                 else {
                     uint64_t sum = 0;
-                    walk(lowest, [&](int, const float *x) {
+                    walk(listed, [&](int, const float *x) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
                             const uint32_t key = key_of(x[j]);
@@ -944,7 +961,7 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
                 const uint64_t amount = (uint64_t)fmax(1.0, ceil(limit));
                 uint32_t t;
                 auto each = [&](auto take) {
-                    walk(lowest, [&](int, const float *x) {
+                    walk(listed, [&](int, const float *x) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j) take(key_of(x[j]), x[j], [&] { return mass_int(x[j]); });
                         return true;
@@ -961,9 +978,9 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
             }
             // what is kept of every group, and how many actions on the threshold come before it
             uint32_t on = 0;
-            const uint32_t need = max(low, tau);
+            listed = list_groups(max(low, tau));
             if (tau > KEY_NONE)
-                walk(need, [&](int, const float *x) {
+                walk(listed, [&](int, const float *x) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) on += key_of(x[j]) == tau;
                     return true;
@@ -977,7 +994,7 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
             uint32_t seen = 0;
 #pragma unroll
             for (int i = 0; i < W; ++i) seen += i < wave ? S.wave_u32[i] : 0;
-            walk(need, [&](int g, const float *x) {
+            walk(listed, [&](int g, const float *x) {
                 uint32_t c = 0;
                 if (tau > KEY_NONE)
 #pragma unroll

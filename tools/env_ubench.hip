@@ -1,5 +1,5 @@
 // env_ubench.hip -- A/B microbenchmark for the env step kernel variants (one process, interleaved rounds).
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 tools/env_ubench.hip -o gpurun_out/env_ubench && ./env_ubench
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 tools/env_ubench.hip -o gpurun_out/env_ubench && ./env_ubench
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdio.h>

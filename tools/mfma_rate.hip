@@ -5,7 +5,7 @@
 //   B  the counted raw barrier per stage
 //   D  one 1-KB LDS-DMA per wave per stage
 // Prints shader cycles per stage (wave 0 of every block, averaged) next to the 16-cycle-per-MFMA ideal.
-//   hipcc --offload-arch=gfx950 -O3 tools/mfma_rate.hip -o tools/mfma_rate.bin
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/mfma_rate.hip -o tools/mfma_rate.bin
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>
