@@ -200,7 +200,7 @@ template <int XD, int E, int WAYS> __device__ __forceinline__ int wave_pick(cons
 #pragma unroll
             for (int k = 0; k < E; ++k) sum += key[k] > tau ? w[k] : 0.0;
             sum = total(sum) + (tau > KEY_NONE ? ties * mass_of(value_of(tau), m, s.c) : 0.0);
-            const double limit = s.top_p * (all > 0.0 ? all : sum);
+            const double limit = lane_of(s.top_p * (all > 0.0 ? all : sum), 0);   // the same in every lane: the search below branches for the whole wave
             // the answer lies in [lo, hi]: the least key that can be kept, and the largest, above which nothing is (in steps of 2^ENDS, which part all keys)
             uint32_t lo = max(least, tau) >> ENDS, hi = top >> ENDS;
             while (lo < hi) {
@@ -217,17 +217,15 @@ template <int XD, int E, int WAYS> __device__ __forceinline__ int wave_pick(cons
                 }
 #pragma unroll
                 for (int i = 0; i < WAYS - 1; ++i) over[i] = scan(over[i]);
-                uint32_t from = lo;
-                bool done = false;
+                uint32_t from = lo, upto = hi;
 #pragma unroll
-                for (int i = 0; i < WAYS - 1; ++i) {
-                    if (done) continue;
-                    if (lane_of(over[i], 63) < limit) {
-                        hi = mid[i];
-                        done = true;
-                    } else from = mid[i] + 1;
+                for (int i = WAYS - 2; i >= 0; --i) {
+                    const bool below = __builtin_amdgcn_readfirstlane(lane_of(over[i], 63) < limit);
+                    upto = below ? mid[i] : upto;
+                    from = !below && from == lo ? mid[i] + 1 : from;
                 }
-                lo = min(from, hi);
+                lo = min(from, upto);
+                hi = upto;
             }
             lo = ENDS ? (lo << ENDS) | (lo << ENDS & 0x80000000u ? 0 : (1u << ENDS) - 1) : lo;
             double above = 0.0;
