@@ -10,10 +10,12 @@
 // All masses are held in 64 bits, because a draw next to the border of two actions has to fall on its own side: at 131,072 actions f32 sums would put
 // one draw in a thousand wrong.  Sums run in a fixed order, or over integers (w scaled to 2^s, so that atomics give the same total in any order).
 //
-// Up to 512 actions: one wave per row.  Up to 8192: one workgroup of 4, 8 or 16 waves per row.  Both hold the row in registers, one launch.
+// Up to 512 actions: one wave per row.  Up to 8192: one workgroup of 4, 8 or 16 waves per row.  Both hold the row in registers, one launch; they are
+// bound by latency (4096 x 65 f32 4.5 us, 256 x 4096 f32 top-p 9 us).
 // Longer rows, two launches: k_sample_groups reads the logits once, across all CUs, and leaves the maximum of every 128 actions and, where the
-// row's settings need the total, their mass.  k_sample_row, a workgroup per row, works from those: bounds on what can be kept leave few groups, it
-// reads only these again, takes the actions above the bound into registers (up to 4096 or 8192) and goes on as for a shorter row.
+// row's settings need the total, their mass (256 x 131072 bf16: without the masses 13 us, the memory's time; with them 30 us, the 64-bit exponentials', which
+// keep the vector ALUs 70 % busy).  k_sample_row, a workgroup per row, works from those: bounds on what can be kept leave few groups, it reads only these
+// again, takes the actions above the bound into registers (up to 4096 or 8192) and goes on as for a shorter row (median row 15 us, bound by the latency of about ten dependent steps).
 #include <math.h>
 #include <algorithm>
 #include <type_traits>
@@ -639,7 +641,8 @@ template <int XD, int W> __global__ void __launch_bounds__(64 * W) k_sample_bloc
 // ---- longer rows ---------------------------------------------------------------------------------------------------------------------
 constexpr int GROUP = 128;          // actions whose maximum and mass are kept together: 16 lanes of 8
 constexpr int MAX_V = 1 << 19;      // 4096 groups
-constexpr int BLOCK_V = 8192;       // the longest row that one workgroup holds in registers from the start
+// rows that one workgroup holds in registers from the start
+inline bool in_block(int64_t n, int64_t v) { return v <= 4096 || (v <= 8192 && n <= 512); }
 
 // whether a row's total mass has to come from all of its actions
 __device__ __forceinline__ bool needs_mass(const Setting &s) { return !s.greedy && !s.k && (s.p_on || !s.m_on); }
@@ -877,7 +880,7 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
                 many += c;
                 start[i + 1] = many;
             }
-            if (most <= SEG && many <= 512) {    // few: one wave goes on without the others
+            if (most <= SEG && many <= 512) {    // few: one wave goes on without the others (4 x 131072 f32, top-k 50 and top-p: 17.9 us; the workgroup together 24.0)
                 if (wave) return;
                 auto finish = [&](auto size) {
                     constexpr int E = decltype(size)::value;
@@ -1095,11 +1098,13 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
 
 template <int XD> int launch(const SampleArgs &A, void *workspace, hipStream_t s) {
     const unsigned rows = (unsigned)A.n;
+    // 4096 x 500 f32, top-p: a wave a row 26.5 us, a workgroup 33.7.  4096 x 2000 f32, top-p: four waves a row 35.6 us, eight 75.6.  4096 x 4096 bf16, top-p: in one launch 74 us,
+    // in two 98.  8192 f32, top-p: 256 rows 14.0 and 24.1 us, 2048 rows 98 and 77.
     if (A.v <= 128) hipLaunchKernelGGL((k_sample_wave<XD, 2>), dim3((rows + 3) / 4), dim3(256), 0, s, A);
     else if (A.v <= 512) hipLaunchKernelGGL((k_sample_wave<XD, 8>), dim3((rows + 3) / 4), dim3(256), 0, s, A);
     else if (A.v <= 2048) hipLaunchKernelGGL((k_sample_block<XD, 4>), dim3(rows), dim3(256), 0, s, A);
     else if (A.v <= 4096) hipLaunchKernelGGL((k_sample_block<XD, 8>), dim3(rows), dim3(512), 0, s, A);
-    else if (A.v <= BLOCK_V) hipLaunchKernelGGL((k_sample_block<XD, 16>), dim3(rows), dim3(1024), 0, s, A);
+    else if (in_block(A.n, A.v)) hipLaunchKernelGGL((k_sample_block<XD, 16>), dim3(rows), dim3(1024), 0, s, A);
     else {
         const int groups = (A.v + GROUP - 1) / GROUP;
         double *mass = (double *)workspace;
@@ -1117,12 +1122,14 @@ template <int XD> int launch(const SampleArgs &A, void *workspace, hipStream_t s
             B.action = A.action + r;
             const double *row_mass = mass + r * groups;
             const uint32_t *row_top = top + r * groups;
-            // four tiles a workgroup share its settings; not where that leaves CUs without one
+            // four tiles a workgroup share its settings; not where that leaves CUs without one (131,072 bf16, no filter, four tiles / one: 4 rows 12.8 / 10.8 us, 64 rows 20.0 / 20.3 us,
+            // 1024 rows 139 / 153 us)
             const bool many = B.n * ((A.v + 8191) / 8192) >= 1024;
             if (many) hipLaunchKernelGGL((k_sample_groups<XD, 4>), dim3((A.v + 8191) / 8192, (unsigned)B.n), dim3(256), 0, s, B, groups, (double *)row_mass, (uint32_t *)row_top);
             else hipLaunchKernelGGL((k_sample_groups<XD, 1>), dim3((A.v + 2047) / 2048, (unsigned)B.n), dim3(256), 0, s, B, groups, (double *)row_mass, (uint32_t *)row_top);
             MZ_LAUNCH_CHECK("k_sample_groups");
-            // up to a row per CU: sixteen waves each; more rows: eight waves each, so that a CU works on two
+            // up to a row per CU: sixteen waves each; more rows: eight waves each, so that a CU works on two (131,072 bf16, sixteen / eight: 256 rows top-p 54 / 54 us, top-k 1000 88 / 123 us;
+            // 400 rows top-p 90 / 82 us, top-k 50 43 / 35 us)
             if (A.n <= 256) hipLaunchKernelGGL((k_sample_row<XD, 16, 8>), dim3((unsigned)B.n), dim3(1024), (size_t)groups * 12, s, B, groups, row_mass, row_top);
             else hipLaunchKernelGGL((k_sample_row<XD, 8, 8>), dim3((unsigned)B.n), dim3(512), (size_t)groups * 12, s, B, groups, row_mass, row_top);
             MZ_LAUNCH_CHECK("k_sample_row");
@@ -1138,7 +1145,7 @@ constexpr int64_t MAX_N = (1 << 22) - 1;
 
 extern "C" int64_t mz_sample_actions_workspace_bytes(int64_t n, int64_t v) {
     if (n < 0 || n > MAX_N || v < 1 || v > MAX_V) return -1;
-    return v <= BLOCK_V ? 0 : std::max<int64_t>(n, 1) * ((v + GROUP - 1) / GROUP) * 12;
+    return in_block(n, v) ? 0 : std::max<int64_t>(n, 1) * ((v + GROUP - 1) / GROUP) * 12;
 }
 
 extern "C" int mz_sample_actions(const mz_sample_args *a, void *workspace, int64_t workspace_bytes, void *stream) {

@@ -77,7 +77,7 @@ def _inputs(n, v, dtype, tdtype, legal, pad, weight, seed):
 
 
 SHAPES = [(1, 1), (1, 65), (6, 2), (3, 64), (7, 128), (4, 129), (9, 512), (6, 513), (5, 1000), (3, 2049), (4, 4097), (3, 8191), (2, 16384), (3, 16391), (2, 40000),
-          (130, 20000), (129, 33001), (131, 65536), (129, 70001), (2, 131072), (1, 200001)]
+          (130, 20000), (129, 33001), (131, 65536), (129, 70001), (2, 131072), (1, 200001), (17, 140001), (3, 70000)]
 
 
 @pytest.mark.parametrize("pair", [(F32, F32), (BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)], ids=str)

@@ -174,13 +174,14 @@ def test_frequencies_follow_the_distribution():
 
 
 @pytest.mark.parametrize("kw", SETTINGS, ids=str)
-@pytest.mark.parametrize("v, dtype", [(9000, F32), (20011, BF16)], ids=str)
+@pytest.mark.parametrize("v, dtype", [(9000, F32), (20011, BF16), (6001, F16)], ids=str)
 def test_more_rows_than_the_card_has_cus(v, dtype, kw):
-    x = (2.5 * torch.randn(300, v, device="cuda", generator=torch.Generator(device="cuda").manual_seed(v))).to(dtype)
+    n = 300 if v > 8192 else 600
+    x = (2.5 * torch.randn(n, v, device="cuda", generator=torch.Generator(device="cuda").manual_seed(v))).to(dtype)
     from muzero_amd.policy import sample_actions
-    u = _uniforms(300, 12)
+    u = _uniforms(n, 12)
     got = sample_actions(x, u, **kw)
-    at = list(range(0, 300, 13))
+    at = list(range(0, n, 23))
     assert got[at].tolist() == _want(x[at], u[at], **kw)
 
 

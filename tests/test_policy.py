@@ -89,7 +89,7 @@ def test_sample_arguments_are_checked_before_any_launch(kw, why):
 def test_sample_workspace_is_checked():
     from muzero_amd import _lib as L
     size = L.lib.mz_sample_actions_workspace_bytes
-    assert size(4, 8192) == 0 and size(4, 8193) == 4 * 65 * 12
+    assert size(4, 8192) == 0 and size(4, 8193) == 4 * 65 * 12 and size(513, 4096) == 0 and size(513, 4097) == 513 * 33 * 12
     for bad in ((-1, 65), (4, 0), (4, (1 << 19) + 1), (1 << 22, 65)):
         assert size(*bad) == -1
     for ws, nbytes, why in ((None, 1 << 30, "workspace"), ((1 << 40) + 4, 1 << 30, "misaligned"), (1 << 40, size(4, 10000) - 1, "needed")):
