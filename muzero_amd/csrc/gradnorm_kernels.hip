@@ -2,12 +2,11 @@
 //
 //   norm = sqrt(sum over tensors and elements of g^2),   dst = src * min(1, max_norm / (norm + 1e-6))
 //
-// Both passes are bound by memory: the norm of 400 M bf16 gradients takes 183 us (4.4 TB/s), their scaling into f32 500 us (4.8 TB/s; a large copy reaches
-// 4.7).  The tensors are cut into chunks of equal bytes and a fixed number of workgroups walks over them, so a list of
-// forty ragged tensors costs what one flat buffer of their size does: one launch per 256 tensors for the norm, per 128 for the scaling.  The list travels in the kernel's
+// Both passes are bound by memory: the norm of 400 M bf16 gradients takes 183 us (4.4 TB/s), their scaling into f32 500 us (4.8 TB/s; a large copy
+// reaches 4.7).  The tensors are cut into chunks of equal bytes and a fixed number of workgroups walks over them, so a list of forty ragged tensors
+// costs what one flat buffer of their size does: one launch per 256 tensors for the norm, per 128 for the scaling.  The list travels in the kernel's
 // arguments (no copy to the device, so a call can be captured).  Squares and sums are held in 64 bits: no overflow above 1.8e19, no underflow below
 // 1e-23, and the order of the sums is fixed by the chunks, so the norm has the same bits on every call.
-#include <stdlib.h>
 #include <algorithm>
 #include <new>
 #include "numeric.h"

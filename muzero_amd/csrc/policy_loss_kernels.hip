@@ -6,10 +6,11 @@
 // A term with t = 0 counts as 0 also where x is -inf.  A row without a legal action, or of weight 0, gives 0 and a zero gradient.
 //
 // Bound by memory: x and t are read, the gradient is written.  So the loss and the gradient come out of ONE pass: the row stays in registers between
-// its sums and its gradient (one wave per row up to 512 actions, one workgroup above), and a training step reads x and t once, not twice: 4096 x 32768 bf16 takes
-// 155 us, 5.2 TB/s, where a large copy reaches 4.7.  Rows that are too long for a workgroup's registers are cut into chunks: one launch for the chunks' sums, one that joins them and writes
-// the gradient (both read x and t: 5 parts of traffic for 3; in slabs of rows that would stay in the last-level cache between the two launches it
-// was slower, 512 x 131072 f32: 310 us in slabs of 96 MB, 263 us without).  Softmax statistics and row sums are f32, sums over rows 64 bits; 16-bit gradients are rounded once.
+// its sums and its gradient (one wave per row up to 512 actions, one workgroup above), and a training step reads x and t once, not twice:
+// 4096 x 32768 bf16 takes 155 us, 5.2 TB/s, where a large copy reaches 4.7.  Rows that are too long for a workgroup's registers are cut into chunks:
+// one launch for the chunks' sums, one that joins them and writes the gradient (both read x and t: 5 parts of traffic for 3; in slabs of rows that
+// would stay in the last-level cache between the two launches it was slower, 512 x 131072 f32: 310 us in slabs of 96 MB, 263 us without).
+// Softmax statistics and row sums are f32, sums over rows 64 bits; 16-bit gradients are rounded once.
 #include <math.h>
 #include <algorithm>
 #include "numeric.h"
@@ -320,17 +321,20 @@ __global__ void __launch_bounds__(1024) k_loss_sum(const float *row_loss, int64_
 constexpr int64_t MAX_V = 1 << 24, MAX_N = (1 << 22) - 1;   // a launch has fewer than 2^32 threads
 
 constexpr int64_t SLAB = 65535;         // rows of one pair of launches: what a grid's second dimension takes
-// Chunks of 8192 actions or more; with few rows of 2048 or more, for more CUs (131,072 f32 actions, in 2048 / 8192: 1 row 14.9 / 19.8 us, 8 rows 17.3 / 20.8 us,
-// 64 rows 47.1 / 40.9 us)
-int chunk_size(int64_t n, int64_t v) { return (int)std::max<int64_t>(n <= 16 ? 2048 : 8192, ((v + CHUNKS - 1) / CHUNKS + 2047) / 2048 * 2048); }
+// Chunks of 8192 actions or more; with few rows of 2048 or more, for more CUs (131,072 f32 actions, in 2048 / 8192: 1 row 14.9 / 19.8 us, 8 rows
+// 17.3 / 20.8 us, 64 rows 47.1 / 40.9 us)
+int chunk_size(int64_t n, int64_t v) {
+    return (int)std::max<int64_t>(n <= 16 ? 2048 : 8192, ((v + CHUNKS - 1) / CHUNKS + 2047) / 2048 * 2048);
+}
 int chunk_count(int64_t n, int64_t v) { return (int)((v + chunk_size(n, v) - 1) / chunk_size(n, v)); }
 
 template <int XD, int TD> int launch(const LossArgs &A, Stat *part, hipStream_t s) {
     constexpr int VEC = Elem<XD>::VEC;
     const unsigned rows = (unsigned)A.n;
     const int64_t vecs = ((int64_t)A.v + VEC - 1) / VEC;
-    // The smallest workgroup whose registers hold a row, so that a CU has several to overlap one's loads with another's stores: 4096 x 500 f32 by a wave 14.1 us, by a
-    // workgroup 16.9; 4096 x 16384 f32 by 512 threads 193 us, by 1024 218; 64 x 16384 f32 by a workgroup 15.2 us, in chunks 20.4; 256 x 32768 f32 32.9 and 41.3.
+    // The smallest workgroup whose registers hold a row, so that a CU has several to overlap one's loads with another's stores: 4096 x 500 f32 by a
+    // wave 14.1 us, by a workgroup 16.9; 4096 x 16384 f32 by 512 threads 193 us, by 1024 218; 64 x 16384 f32 by a workgroup 15.2 us, in chunks 20.4;
+    // 256 x 32768 f32 32.9 and 41.3.
     if (A.v <= 128) hipLaunchKernelGGL((k_loss_wave<XD, TD, 2>), dim3((rows + 3) / 4), dim3(256), 0, s, A);
     else if (A.v <= 512) hipLaunchKernelGGL((k_loss_wave<XD, TD, 8>), dim3((rows + 3) / 4), dim3(256), 0, s, A);
     else if (vecs <= 256 * 2) hipLaunchKernelGGL((k_loss_row<XD, TD, 256, 2>), dim3(rows), dim3(256), 0, s, A);

@@ -15,7 +15,8 @@
 // Longer rows, two launches: k_sample_groups reads the logits once, across all CUs, and leaves the maximum of every 128 actions and, where the
 // row's settings need the total, their mass (256 x 131072 bf16: without the masses 13 us, the memory's time; with them 30 us, the 64-bit exponentials', which
 // keep the vector ALUs 70 % busy).  k_sample_row, a workgroup per row, works from those: bounds on what can be kept leave few groups, it reads only these
-// again, takes the actions above the bound into registers (up to 4096 or 8192) and goes on as for a shorter row (median row 15 us, bound by the latency of about ten dependent steps).
+// again, takes the actions above the bound into registers (up to 4096 or 8192) and goes on as for a shorter row (median row 15 us, bound by the
+// latency of about ten dependent steps).
 #include <math.h>
 #include <algorithm>
 #include <type_traits>
@@ -105,7 +106,9 @@ template <bool FINE> __device__ __forceinline__ double exp2_neg(double t) {
 template <bool FINE = true> __device__ __forceinline__ double mass_of(float x, double m, double c) { return exp2_neg<FINE>(((double)x - m) * c); }
 
 // ---- reductions and scans over a wave in registers: rows of 16 lanes by shifts, then across the rows (lanes that get nothing add 0) ----------
-template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false); }
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
 template <int CTRL, int ROWS> __device__ __forceinline__ double dpp(double v) {
     const uint64_t b = (uint64_t)__double_as_longlong(v);
     return __longlong_as_double((long long)((uint64_t)dpp<CTRL, ROWS>((uint32_t)(b >> 32)) << 32 | dpp<CTRL, ROWS>((uint32_t)b)));
@@ -405,7 +408,9 @@ template <int W> __device__ __forceinline__ int crossing_bin(Shared<W> &S, uint6
 // not matter.  `guess` >= lo: where tau is looked for first; `ends` = bits of a key that its type leaves empty.
 // The first histogram, from `guess` on, has bins of equal width in the value, which few logits share; the up to 64 of the bin that reaches the limit
 // are ranked in registers.  More (equal logits), or tau below the guess: histograms over the keys' bits, each narrowing to one bin of the one before.
-template <int W, class EACH> __device__ __forceinline__ bool find_threshold(EACH each, uint32_t lo, uint32_t guess, uint32_t hi, uint64_t limit, int ends, Shared<W> &S, uint32_t *tau, uint64_t *above_out) {
+template <int W, class EACH>
+__device__ __forceinline__ bool find_threshold(EACH each, uint32_t lo, uint32_t guess, uint32_t hi, uint64_t limit, int ends, Shared<W> &S,
+                                               uint32_t *tau, uint64_t *above_out) {
     constexpr int BINS = Shared<W>::BINS, BITS = W == 4 ? 10 : W == 8 ? 11 : 12, FEW = Shared<W>::FEW;
     static_assert(1 << BITS == BINS, "a bin for each key of that many bits");
     const int lane = threadIdx.x & 63;
@@ -487,7 +492,8 @@ __device__ __forceinline__ uint64_t int_mass(double w, double scale) {   // the 
 
 // The answer for what the workgroup's threads hold in registers, thread by thread in the actions' order, N in each: the place of the picked one
 // (thread N + j), in every thread.  best: the largest key.  low: nothing below it is kept.  all: the mass that top-p shares out, if it is known (> 0).
-template <int XD, int W, int N> __device__ __forceinline__ int pick(const float *x, const Setting &s, double u, int v, uint32_t best, uint32_t low, double all, Shared<W> &S) {
+template <int XD, int W, int N>
+__device__ __forceinline__ int pick(const float *x, const Setting &s, double u, int v, uint32_t best, uint32_t low, double all, Shared<W> &S) {
     constexpr int ENDS = key_ends<XD>();
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const double m = (double)value_of(best);
@@ -880,7 +886,8 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
                 many += c;
                 start[i + 1] = many;
             }
-            if (most <= SEG && many <= 512) {    // few: one wave goes on without the others (4 x 131072 f32, top-k 50 and top-p: 17.9 us; the workgroup together 24.0)
+            // few: one wave goes on without the others (4 x 131072 f32, top-k 50 and top-p: 17.9 us; the workgroup together 24.0)
+            if (most <= SEG && many <= 512) {
                 if (wave) return;
                 auto finish = [&](auto size) {
                     constexpr int E = decltype(size)::value;
@@ -975,7 +982,7 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
                         tau = t;
                         ties = r;
                     } else ties = min(ties, r);
-                }
+                } else if (tau <= KEY_NONE) tau = low - 1;   // rounding: everything from `low` on
             }
             // what is kept of every group, and how many actions on the threshold come before it
             uint32_t on = 0;
@@ -1098,8 +1105,8 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
 
 template <int XD> int launch(const SampleArgs &A, void *workspace, hipStream_t s) {
     const unsigned rows = (unsigned)A.n;
-    // 4096 x 500 f32, top-p: a wave a row 26.5 us, a workgroup 33.7.  4096 x 2000 f32, top-p: four waves a row 35.6 us, eight 75.6.  4096 x 4096 bf16, top-p: in one launch 74 us,
-    // in two 98.  8192 f32, top-p: 256 rows 14.0 and 24.1 us, 2048 rows 98 and 77.
+    // top-p, 4096 x 500 f32: a wave a row 26.5 us, a workgroup 33.7.  4096 x 2000 f32: four waves a row 35.6 us, eight 75.6.  4096 x 4096 bf16: in one
+    // launch 74 us, in two 98.  8192 f32: 256 rows 14.0 and 24.1 us, 2048 rows 98 and 77.
     if (A.v <= 128) hipLaunchKernelGGL((k_sample_wave<XD, 2>), dim3((rows + 3) / 4), dim3(256), 0, s, A);
     else if (A.v <= 512) hipLaunchKernelGGL((k_sample_wave<XD, 8>), dim3((rows + 3) / 4), dim3(256), 0, s, A);
     else if (A.v <= 2048) hipLaunchKernelGGL((k_sample_block<XD, 4>), dim3(rows), dim3(256), 0, s, A);
@@ -1120,18 +1127,23 @@ template <int XD> int launch(const SampleArgs &A, void *workspace, hipStream_t s
             if (A.top_p_of) B.top_p_of = A.top_p_of + r;
             if (A.min_p_of) B.min_p_of = A.min_p_of + r;
             B.action = A.action + r;
-            const double *row_mass = mass + r * groups;
-            const uint32_t *row_top = top + r * groups;
-            // four tiles a workgroup share its settings; not where that leaves CUs without one (131,072 bf16, no filter, four tiles / one: 4 rows 12.8 / 10.8 us, 64 rows 20.0 / 20.3 us,
-            // 1024 rows 139 / 153 us)
+            double *row_mass = mass + r * groups;
+            uint32_t *row_top = top + r * groups;
+            // four tiles a workgroup share its settings; not where that leaves CUs without one (131,072 bf16, no filter, four tiles / one: 4 rows
+            // 12.8 / 10.8 us, 64 rows 20.0 / 20.3 us, 1024 rows 139 / 153 us)
             const bool many = B.n * ((A.v + 8191) / 8192) >= 1024;
-            if (many) hipLaunchKernelGGL((k_sample_groups<XD, 4>), dim3((A.v + 8191) / 8192, (unsigned)B.n), dim3(256), 0, s, B, groups, (double *)row_mass, (uint32_t *)row_top);
-            else hipLaunchKernelGGL((k_sample_groups<XD, 1>), dim3((A.v + 2047) / 2048, (unsigned)B.n), dim3(256), 0, s, B, groups, (double *)row_mass, (uint32_t *)row_top);
+            if (many)
+                hipLaunchKernelGGL((k_sample_groups<XD, 4>), dim3((A.v + 8191) / 8192, (unsigned)B.n), dim3(256), 0, s, B, groups, row_mass, row_top);
+            else
+                hipLaunchKernelGGL((k_sample_groups<XD, 1>), dim3((A.v + 2047) / 2048, (unsigned)B.n), dim3(256), 0, s, B, groups, row_mass, row_top);
             MZ_LAUNCH_CHECK("k_sample_groups");
-            // up to a row per CU: sixteen waves each; more rows: eight waves each, so that a CU works on two (131,072 bf16, sixteen / eight: 256 rows top-p 54 / 54 us, top-k 1000 88 / 123 us;
-            // 400 rows top-p 90 / 82 us, top-k 50 43 / 35 us)
-            if (A.n <= 256) hipLaunchKernelGGL((k_sample_row<XD, 16, 8>), dim3((unsigned)B.n), dim3(1024), (size_t)groups * 12, s, B, groups, row_mass, row_top);
-            else hipLaunchKernelGGL((k_sample_row<XD, 8, 8>), dim3((unsigned)B.n), dim3(512), (size_t)groups * 12, s, B, groups, row_mass, row_top);
+            // up to a row per CU: sixteen waves each; more rows: eight waves each, so that a CU works on two (131,072 bf16, sixteen / eight: 256 rows top-p
+            // 54 / 54 us, top-k 1000 88 / 123 us; 400 rows top-p 90 / 82 us, top-k 50 43 / 35 us)
+            const size_t lds = (size_t)groups * 12;
+            const double *m = row_mass;
+            const uint32_t *t = row_top;
+            if (A.n <= 256) hipLaunchKernelGGL((k_sample_row<XD, 16, 8>), dim3((unsigned)B.n), dim3(1024), lds, s, B, groups, m, t);
+            else hipLaunchKernelGGL((k_sample_row<XD, 8, 8>), dim3((unsigned)B.n), dim3(512), lds, s, B, groups, m, t);
             MZ_LAUNCH_CHECK("k_sample_row");
         }
     }
@@ -1156,7 +1168,8 @@ extern "C" int mz_sample_actions(const mz_sample_args *a, void *workspace, int64
     MZ_REQUIRE(elem_known(a->dtype), "%s: unknown dtype %d", who, a->dtype);
     MZ_REQUIRE(!a->board || a->v == 65, "%s: a bitboard needs v = 65", who);
     MZ_REQUIRE(!(a->board && a->allowed), "%s: allowed or board, not both", who);
-    MZ_REQUIRE(a->temperature_of || a->temperature == 0.0 || (a->temperature >= 1e-30 && a->temperature <= 1e30), "%s: the temperature has to be 0, or 1e-30 .. 1e30", who);
+    MZ_REQUIRE(a->temperature_of || a->temperature == 0.0 || (a->temperature >= 1e-30 && a->temperature <= 1e30),
+               "%s: the temperature has to be 0, or 1e-30 .. 1e30", who);
     MZ_REQUIRE(a->top_k_of || a->top_k >= 0, "%s: top_k has to be 0 (off) or more", who);
     MZ_REQUIRE(a->top_p_of || (a->top_p >= 0.0 && a->top_p <= 1.0), "%s: top_p has to be in [0, 1]", who);
     MZ_REQUIRE(a->min_p_of || (a->min_p >= 0.0 && a->min_p <= 1.0), "%s: min_p has to be in [0, 1]", who);

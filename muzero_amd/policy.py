@@ -37,7 +37,8 @@ def _rows(who, name, t, shape=None, dtypes=tuple(_DT)):
 
 def _per_row(who, name, t, n, dtype, dev):
     if not t.is_cuda or t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or t.device != dev:
-        raise L.MzError("%s: %s has to be a contiguous %s tensor of shape (%d,) on %s, got %s %s on %s" % (who, name, dtype, n, dev, tuple(t.shape), t.dtype, t.device))
+        raise L.MzError("%s: %s has to be a contiguous %s tensor of shape (%d,) on %s, got %s %s on %s"
+                        % (who, name, dtype, n, dev, tuple(t.shape), t.dtype, t.device))
     return t.data_ptr()
 
 
@@ -181,8 +182,8 @@ def sample_actions(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, le
     else:
         _per_row(who, "out", out, n, torch.int32, dev)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    args = _SAMPLE_ARGS(logits.data_ptr(), allowed, board, u_ptr, temperature_of, top_k_of, top_p_of, min_p_of, out.data_ptr(), n, v, stride, allowed_stride, int(top_k),
-                        temperature, top_p, min_p, _DT[logits.dtype])
+    args = _SAMPLE_ARGS(logits.data_ptr(), allowed, board, u_ptr, temperature_of, top_k_of, top_p_of, min_p_of, out.data_ptr(), n, v, stride,
+                        allowed_stride, int(top_k), temperature, top_p, min_p, _DT[logits.dtype])
     L.call_on(dev.index, "mz_sample_actions", args, None if ws is None else ws.data_ptr(), nbytes)
     torch.autograd.graph.increment_version(out)
     return out
