@@ -75,9 +75,9 @@ constexpr uint32_t KEY_INF = 0xFF800000u;      // +inf, and above it NaN: no dis
 
 // 2^t for t <= 0: 2^round(t) times a polynomial at f = t - round(t) in [-1/2, 1/2], 1 + f q(f) with q the interpolation of (2^f - 1) / f at the
 // Chebyshev nodes (2^0 is 1 exactly): of degree 9, relative error 6e-16, or where FINE is false of degree 7, 2e-12.  Adding 1.5 2^52 rounds t and
-// leaves the integer in the low word.  Below 2^-1000 the answer is 2^-1000: next to the row's best, whose mass is 1, nothing.
+// leaves the integer in the low word.  Below 2^-1075 it is 0, as any 64-bit exponential: u = 0 takes none of those.
 template <bool FINE> __device__ __forceinline__ double exp2_neg(double t) {
-    t = fmax(t, -1000.0);
+    t = fmax(t, -1100.0);
     const double big = 6755399441055744.0, r = t + big, f = t - (r - big);
     double q;
     if (FINE) {

@@ -185,6 +185,16 @@ def test_more_rows_than_the_card_has_cus(v, dtype, kw):
     assert got[at].tolist() == _want(x[at], u[at], **kw)
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=60), dict(top_k=1000), dict(top_p=0.9), dict(min_p=1e-9)], ids=str)
+@pytest.mark.parametrize("v", [65, 400, 2000, 5000, 9001, 131072])
+def test_a_uniform_of_zero_takes_no_action_whose_mass_is_zero(v, kw):
+    """e^-2000 is 0 in 64 bits; e^-600 is not"""
+    x, u = torch.zeros(2, v, device="cuda"), torch.zeros(2, dtype=torch.float64, device="cuda")
+    x[0, v - 2], x[1, v - 2] = 2000.0, 600.0
+    got = _check(x, u, **kw).tolist()
+    assert got == [v - 2, 0 if "top_p" not in kw and "min_p" not in kw else v - 2]
+
+
 def test_many_rows_and_the_largest_vocabulary():
     g = torch.Generator(device="cuda").manual_seed(9)
     x = torch.randn(1, 2 ** 19, device="cuda", generator=g) * 3
