@@ -849,42 +849,79 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
                     }
                 }
             };
-            // the actions from `low` on, in their order, each wave's in a segment of its own
-            int count = 0;
-            int listed = list_groups(low);
-            if (bounded) {
-                const float least = value_of(low);
-                walk(listed, [&](int g, const float *x) {
-                    uint32_t n = 0;
+            // where the k-th is looked for first: `low` or, without a bound, twice as far below the best as the least of the groups' maxima
+            auto first_guess = [&]() -> uint32_t {
+                if (bounded) return low;
+                uint32_t least = 0xFFFFFFFFu;
+                for (int g = threadIdx.x; g < groups; g += THREADS)
+                    if (top[g] > KEY_NONE) least = min(least, top[g]);
+                least = ~block_max<W>(~least, S.wave_u32);
+                return bound(m - 2.0 * (m - (double)value_of(least)));
+            };
+            // The actions from `low` on, in their order, each wave's in a segment of its own.  Too many (or no bound yet) where top-k keeps at most half of
+            // what fits: the k-th largest's place in a histogram of the values is a closer bound, and once more (k = 2000, that / the row read again
+            // for each step: 256 x 131072 bf16 64 / 118 us, 64 x 10000 f32 25 / 30 us).
+            int count, listed, many, most, start[W + 1];
+            for (bool closer = false;;) {
+                count = 0;
+                listed = list_groups(low);
+                if (bounded) {
+                    const float least = value_of(low);
+                    walk(listed, [&](int g, const float *x) {
+                        uint32_t n = 0;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) n += x[j] >= least;
-                    const uint32_t upto = scan(n);
-                    int to = count + (int)(upto - n);
-                    count += (int)lane_of(upto, 63);
+                        for (int j = 0; j < 8; ++j) n += x[j] >= least;
+                        const uint32_t upto = scan(n);
+                        int to = count + (int)(upto - n);
+                        count += (int)lane_of(upto, 63);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (x[j] >= least) {
+                                if (to < SEG) {
+                                    R.x[wave * SEG + to] = x[j];
+                                    R.index[wave * SEG + to] = g * GROUP + (lane & 15) * 8 + j;
+                                }
+                                ++to;
+                            }
+                        return count <= SEG;
+                    });
+                }
+                __syncthreads();
+                if (lane == 0) S.wave_u32[wave] = bounded ? (uint32_t)count : SEG + 1u;
+                __syncthreads();
+                many = most = start[0] = 0;
+                const uint32_t of_wave = lane < W ? S.wave_u32[lane] : 0;
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    const int c = (int)lane_of(of_wave, i);
+                    most = max(most, c);
+                    many += c;
+                    start[i + 1] = many;
+                }
+                if (most <= SEG || closer || !s.k || s.k > W * SEG / 2) break;
+                closer = true;
+                __syncthreads();                 // wave_u32 is used again
+                constexpr int BINS = Shared<W>::BINS;
+                const uint32_t from = first_guess();
+                const float high = value_of(best), width = high - value_of(from), scale = BINS / width;
+                if (!(scale > 0.0f && scale < 1e30f)) break;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) S.hist[threadIdx.x * 4 + i] = 0;
+                if (threadIdx.x == 0) S.bin = -1;
+                __syncthreads();
+                walk(listed, [&](int, const float *x) {
+                    const float least = value_of(from);
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        if (x[j] >= least) {
-                            if (to < SEG) {
-                                R.x[wave * SEG + to] = x[j];
-                                R.index[wave * SEG + to] = g * GROUP + (lane & 15) * 8 + j;
-                            }
-                            ++to;
-                        }
-                    return count <= SEG;
+                        if (x[j] >= least) atomicAdd(&S.hist[min(BINS - 1, (int)((high - x[j]) * scale))], 1ull);
+                    return true;
                 });
-            }
-            __syncthreads();
-            if (lane == 0) S.wave_u32[wave] = bounded ? (uint32_t)count : SEG + 1u;
-            __syncthreads();
-            int many = 0, most = 0, start[W + 1];
-            start[0] = 0;
-            const uint32_t of_wave = lane < W ? S.wave_u32[lane] : 0;
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-                const int c = (int)lane_of(of_wave, i);
-                most = max(most, c);
-                many += c;
-                start[i + 1] = many;
+                __syncthreads();
+                uint64_t above = 0;
+                const int bin = crossing_bin(S, (uint64_t)s.k, &above);
+                if (bin < 0) break;
+                low = bound((double)high - (bin + 1.0) / BINS * (double)width);
+                bounded = true;
             }
             // few: one wave goes on without the others (4 x 131072 f32, top-k 50 and top-p: 17.9 us; the workgroup together 24.0)
             if (most <= SEG && many <= 512) {
@@ -934,15 +971,7 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
                         return true;
                     });
                 };
-                uint32_t guess = low;
-                if (!bounded) {                  // twice as far below the best as the least of the groups' maxima
-                    uint32_t least = 0xFFFFFFFFu;
-                    for (int g = threadIdx.x; g < groups; g += THREADS)
-                        if (top[g] > KEY_NONE) least = min(least, top[g]);
-                    least = ~block_max<W>(~least, S.wave_u32);
-                    guess = bound(m - 2.0 * (m - (double)value_of(least)));
-                }
-                if (find_threshold(each, low, guess, best, (uint64_t)s.k, ENDS, S, &t, &above)) {
+                if (find_threshold(each, low, first_guess(), best, (uint64_t)s.k, ENDS, S, &t, &above)) {
                     tau = t;
                     ties = (uint32_t)(s.k - above);
                 }

@@ -185,6 +185,35 @@ def test_more_rows_than_the_card_has_cus(v, dtype, kw):
     assert got[at].tolist() == _want(x[at], u[at], **kw)
 
 
+@pytest.mark.parametrize("k", [200, 700, 1000, 2048, 2049, 4096, 4097])
+@pytest.mark.parametrize("kind", ["spread", "integers", "one peak", "few legal", "equal", "huge", "steps"])
+@pytest.mark.parametrize("n, v, dtype", [(3, 8193, F32), (3, 65537, F32), (2, 131072, BF16), (300, 9001, F16)], ids=str)
+def test_many_of_the_best_in_long_rows(n, v, dtype, kind, k):
+    """the k-th largest far inside the row, among equal ones, behind one far ahead of the others, or not there"""
+    from muzero_amd.policy import sample_actions
+    g = torch.Generator(device="cuda").manual_seed(v + k)
+    x, legal = torch.randn(n, v, device="cuda", generator=g) * 2, None
+    if kind == "integers":
+        x = x.round()
+    elif kind == "one peak":
+        x[:, 77] = 40.0
+    elif kind == "few legal":
+        legal = torch.zeros(n, v, dtype=torch.bool, device="cuda")
+        legal[:, 5::v // 600] = True
+    elif kind == "equal":
+        x.zero_()
+    elif kind == "huge":
+        x[:, 5] = 6e4
+        x[:, 9] = -6e4
+    elif kind == "steps":                        # sorted: the best are next to each other
+        x = x.sort(dim=1).values
+    x, u = x.to(dtype), _uniforms(n, k)
+    at = list(range(0, n, max(1, n // 9)))
+    for kw in (dict(), dict(top_p=0.8, temperature=2.0), dict(min_p=0.03)):
+        got = sample_actions(x, u, top_k=k, legal=legal, **kw)
+        assert got[at].tolist() == _want(x[at], u[at], legal=None if legal is None else legal[at], top_k=k, **kw), kw
+
+
 @pytest.mark.parametrize("kw", [dict(), dict(top_k=60), dict(top_k=1000), dict(top_p=0.9), dict(min_p=1e-9)], ids=str)
 @pytest.mark.parametrize("v", [65, 400, 2000, 5000, 9001, 131072])
 def test_a_uniform_of_zero_takes_no_action_whose_mass_is_zero(v, kw):
