@@ -407,7 +407,8 @@ template <int W> __device__ __forceinline__ int crossing_bin(Shared<W> &S, uint6
 // its argument; *above = that amount.  False: all of it together stays below the limit.  Amounts are integers, so the order of the atomics does
 // not matter.  `guess` >= lo: where tau is looked for first; `ends` = bits of a key that its type leaves empty.
 // The first histogram, from `guess` on, has bins of equal width in the value, which few logits share; the up to 64 of the bin that reaches the limit
-// are ranked in registers.  More (equal logits), or tau below the guess: histograms over the keys' bits, each narrowing to one bin of the one before.
+// are ranked in registers.  More: histograms over the bits of that bin's keys, each narrowing to one bin of the one before, unless they are all equal
+// (256 x 131072 bf16, flat, p = 0.9: 189 us; from all keys 259).  Tau below the guess: the same from all keys.
 template <int W, class EACH>
 __device__ __forceinline__ bool find_threshold(EACH each, uint32_t lo, uint32_t guess, uint32_t hi, uint64_t limit, int ends, Shared<W> &S,
                                                uint32_t *tau, uint64_t *above_out) {
@@ -435,9 +436,12 @@ __device__ __forceinline__ bool find_threshold(EACH each, uint32_t lo, uint32_t 
         __syncthreads();
         const int bin = crossing_bin(S, limit, &above);
         if (bin < 0 && guess == lo) return false;
+        uint32_t least = 0xFFFFFFFFu, most = 0;
         if (bin >= 0) each([&](uint32_t key, float x, auto amount) {
             if (key >= guess && key <= hi && bin_of(x) == bin) {
                 const int i = atomicAdd(&S.few, 1);
+                least = min(least, key);
+                most = max(most, key);
                 if (i < FEW) {
                     S.few_key[i] = key;
                     S.few_amount[i] = (unsigned long long)amount();
@@ -460,7 +464,15 @@ __device__ __forceinline__ bool find_threshold(EACH each, uint32_t lo, uint32_t 
             *above_out = lane_of(over, __ffsll((unsigned long long)__ballot(best == *tau)) - 1);
             return true;
         }
-        above = 0;
+        if (bin >= 0) {           // above: what lies above the bin
+            lo = ~block_max<W>(~least, S.wave_u32);
+            hi = block_max<W>(most, S.wave_u32);
+            if (lo == hi) {
+                *tau = lo;
+                *above_out = above;
+                return true;
+            }
+        }
     }
     for (;;) {
         const int shift = max(0, 32 - __clz((int)(hi - lo)) - BITS);   // (hi - lo) >> shift < BINS
