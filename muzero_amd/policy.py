@@ -55,13 +55,24 @@ def _legal(who, legal, logits):
     return legal.data_ptr(), _rows(who, "legal", legal, logits.shape, (torch.bool,)), 0
 
 
+def _places(who, logits, targets, weight, legal):
+    """-> what a call of the loss reads: the addresses and the rows' strides"""
+    stride = _rows(who, "logits", logits)
+    targets_stride = _rows(who, "targets", targets, logits.shape, (logits.dtype, torch.float32))
+    if targets.device != logits.device:
+        raise L.MzError("%s: targets are on %s, the logits on %s" % (who, targets.device, logits.device))
+    weight_ptr = 0 if weight is None else _per_row(who, "weight", weight, logits.shape[0], torch.float32, logits.device)
+    allowed, allowed_stride, board = _legal(who, legal, logits)
+    return (logits.data_ptr(), targets.data_ptr(), allowed, board, weight_ptr), (stride, targets_stride, allowed_stride)
+
+
 class _CrossEntropy(torch.autograd.Function):
     """The gradient comes out of the forward pass over the rows, for a loss whose own gradient is 1 (what loss.backward() starts
     from).  backward launches the same kernel with the gradient it is given: where that is 1 the kernel leaves at once, otherwise it
     computes the rows again, so a scaled 16-bit gradient is rounded once, after the scale."""
 
     @staticmethod
-    def forward(ctx, logits, targets, weight, legal, reduction, head, tail):
+    def forward(ctx, logits, targets, weight, legal, reduction, head, sizes, strides, rest):
         n, v = logits.shape
         dev = logits.device
         need = ctx.needs_input_grad[0]
@@ -72,7 +83,7 @@ class _CrossEntropy(torch.autograd.Function):
         grad = None
         if need:
             ctx.save_for_backward(logits, targets, weight, legal)
-            ctx.call = head, tail, nbytes
+            ctx.call = sizes, rest, nbytes
             if reduction != "none":
                 grad = torch.empty((n, v), dtype=logits.dtype, device=dev)
             ctx.ready = grad
@@ -81,7 +92,7 @@ class _CrossEntropy(torch.autograd.Function):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         to = out.data_ptr()
         rows, loss = (to, 0) if reduction == "none" else (0, to)
-        L.call_on(dev.index, "mz_policy_loss", _LOSS_ARGS(*head, 0, rows, loss, 0 if grad is None else grad.data_ptr(), *tail, 0, 0), ws.data_ptr(), nbytes)
+        L.call_on(dev.index, "mz_policy_loss", _LOSS_ARGS(*head, 0, rows, loss, 0 if grad is None else grad.data_ptr(), *sizes, *strides, *rest, 0, 0), ws.data_ptr(), nbytes)
         return out
 
     @staticmethod
@@ -89,20 +100,23 @@ class _CrossEntropy(torch.autograd.Function):
         if torch.is_grad_enabled():            # create_graph: the gradient, and an error when its own is asked for
             with torch.no_grad():
                 grad = _CrossEntropy.backward(ctx, go)[0]
-            return _NoSecondDerivative.apply(grad.detach().requires_grad_()), None, None, None, None, None, None
-        logits = ctx.saved_tensors[0]          # also says if one of them was changed in place
+            return (_NoSecondDerivative.apply(grad.detach().requires_grad_()),) + (None,) * 9
+        # also says if one of them was changed in place.  Where hooks pack saved tensors (kept on the host, or computed again) these are new ones
+        # with strides of their own: nothing of the forward's addresses is used here
+        logits, targets, weight, legal = ctx.saved_tensors
         grad = ctx.ready
         ctx.ready = None                       # handed out once; a second backward pass gets memory of its own
         skip = grad is not None
         if grad is None:
             grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         if logits.shape[0]:
-            head, tail, nbytes = ctx.call
+            head, strides = _places("cross_entropy", logits, targets, weight, legal)
+            sizes, rest, nbytes = ctx.call
             if not go.is_contiguous():
                 go = go.contiguous()
             ws = torch.empty(nbytes, dtype=torch.uint8, device=grad.device)   # not the forward's: a captured backward keeps its own
-            L.call_on(grad.get_device(), "mz_policy_loss", _LOSS_ARGS(*head, go.data_ptr(), 0, 0, grad.data_ptr(), *tail, go.dim(), skip), ws.data_ptr(), nbytes)
-        return grad, None, None, None, None, None, None
+            L.call_on(grad.get_device(), "mz_policy_loss", _LOSS_ARGS(*head, go.data_ptr(), 0, 0, grad.data_ptr(), *sizes, *strides, *rest, go.dim(), skip), ws.data_ptr(), nbytes)
+        return (grad,) + (None,) * 9
 
 
 class _NoSecondDerivative(torch.autograd.Function):
@@ -124,21 +138,14 @@ def cross_entropy(logits, targets, weight=None, legal=None, reduction="mean"):
     but gives no loss and no gradient, whatever it holds.  legal: see the module; other places are never used, their gradient is 0,
     and a row without a legal action gives 0.  Targets of 0 count as 0 also against a logit of -inf."""
     who = "cross_entropy"
-    stride = _rows(who, "logits", logits)
-    dtype = logits.dtype
-    targets_stride = _rows(who, "targets", targets, logits.shape, (dtype, torch.float32))
-    if targets.device != logits.device:
-        raise L.MzError("%s: targets are on %s, the logits on %s" % (who, targets.device, logits.device))
     if targets.requires_grad or (weight is not None and weight.requires_grad):
         raise L.MzError("%s: targets and weights carry no gradient (detach them)" % who)
-    n, v = logits.shape
-    weight_ptr = 0 if weight is None else _per_row(who, "weight", weight, n, torch.float32, logits.device)
-    allowed, allowed_stride, board = _legal(who, legal, logits)
+    head, strides = _places(who, logits, targets, weight, legal)
     if reduction not in ("mean", "sum", "none"):
         raise L.MzError("%s: reduction is 'mean', 'sum' or 'none', got %r" % (who, reduction))
-    head = logits.data_ptr(), targets.data_ptr(), allowed, board, weight_ptr
-    tail = n, v, stride, targets_stride, allowed_stride, v, 1.0 / n if reduction == "mean" and n else 1.0, _DT[dtype], _DT[targets.dtype]
-    return _CrossEntropy.apply(logits, targets, weight, legal, reduction, head, tail)
+    n, v = logits.shape
+    rest = v, 1.0 / n if reduction == "mean" and n else 1.0, _DT[logits.dtype], _DT[targets.dtype]
+    return _CrossEntropy.apply(logits, targets, weight, legal, reduction, head, (n, v), strides, rest)
 
 
 def _setting(who, name, value, n, dtype, dev, low, high):

@@ -226,6 +226,30 @@ def test_changed_logits_are_noticed():
         loss.backward()
 
 
+@pytest.mark.parametrize("legal", ["none", "bool"])
+@pytest.mark.parametrize("n, v", [(40, 65), (9, 5003), (3, 70001)])
+def test_saved_tensors_that_come_back_elsewhere(n, v, legal):
+    """between forward and backward the inputs are kept on the host, or computed again: other addresses and other strides"""
+    from torch.utils.checkpoint import checkpoint
+    from muzero_amd.policy import cross_entropy
+    x, t, w, lm = _inputs(n, v, BF16, F32, legal, 7, True, seed=v)
+    want, = torch.autograd.grad(cross_entropy(x, t, w, lm) * 3.0, x)
+    leaf = x.detach().clone().requires_grad_()
+
+    def loss(leaf):
+        wide = torch.nn.functional.pad(leaf, (2, 5))
+        return cross_entropy(wide[:, 2:2 + v], t.clone(), w.clone(), None if lm is None else lm.clone()) * 3.0
+
+    with torch.autograd.graph.save_on_cpu():
+        kept = loss(leaf)
+    again = checkpoint(loss, leaf, use_reentrant=False)
+    for total in (kept, again):
+        junk = [torch.full((n, v + 7), math.nan, dtype=d, device="cuda") for d in (BF16, BF16, F32, F32)]   # where the inputs were
+        got, = torch.autograd.grad(total, leaf)
+        del junk
+        assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("v", [65, 5000, 70001])
 def test_rows_that_share_their_memory(v):
     """one row of logits and one mask for all: their gradients add up"""
