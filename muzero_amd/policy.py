@@ -83,7 +83,7 @@ class _CrossEntropy(torch.autograd.Function):
         grad = None
         if need:
             ctx.save_for_backward(logits, targets, weight, legal)
-            ctx.call = sizes, rest, nbytes
+            ctx.call = head, sizes, strides, rest, nbytes
             if reduction != "none":
                 grad = torch.empty((n, v), dtype=logits.dtype, device=dev)
             ctx.ready = grad
@@ -101,17 +101,20 @@ class _CrossEntropy(torch.autograd.Function):
             with torch.no_grad():
                 grad = _CrossEntropy.backward(ctx, go)[0]
             return (_NoSecondDerivative.apply(grad.detach().requires_grad_()),) + (None,) * 9
-        # also says if one of them was changed in place.  Where hooks pack saved tensors (kept on the host, or computed again) these are new ones
-        # with strides of their own: nothing of the forward's addresses is used here
-        logits, targets, weight, legal = ctx.saved_tensors
+        logits, targets, weight, legal = ctx.saved_tensors   # also says if one of them was changed in place
         grad = ctx.ready
         ctx.ready = None                       # handed out once; a second backward pass gets memory of its own
         skip = grad is not None
         if grad is None:
             grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         if logits.shape[0]:
-            head, strides = _places("cross_entropy", logits, targets, weight, legal)
-            sizes, rest, nbytes = ctx.call
+            head, sizes, strides, rest, nbytes = ctx.call
+            # Where hooks pack saved tensors (kept on the host, or computed again) these are new ones with strides of their own.  (Asking for all
+            # places anew takes 8 us of a pass's 90, the question whether it is needed 1.)
+            if (logits.data_ptr() != head[0] or targets.data_ptr() != head[1] or logits.stride() != (strides[0], 1) or targets.stride() != (strides[1], 1)
+                    or (weight is not None and weight.data_ptr() != head[4])
+                    or (legal is not None and (legal.data_ptr() != (head[2] or head[3]) or (head[2] and legal.stride() != (strides[2], 1))))):
+                head, strides = _places("cross_entropy", logits, targets, weight, legal)
             if not go.is_contiguous():
                 go = go.contiguous()
             ws = torch.empty(nbytes, dtype=torch.uint8, device=grad.device)   # not the forward's: a captured backward keeps its own
