@@ -97,11 +97,17 @@ class _CrossEntropy(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, go):
+        saved = ctx.saved_tensors              # also says if one of them was changed in place; asked for once, as recomputed ones have to be
         if torch.is_grad_enabled():            # create_graph: the gradient, and an error when its own is asked for
             with torch.no_grad():
-                grad = _CrossEntropy.backward(ctx, go)[0]
-            return (_NoSecondDerivative.apply(grad.detach().requires_grad_()),) + (None,) * 9
-        logits, targets, weight, legal = ctx.saved_tensors   # also says if one of them was changed in place
+                grad = _CrossEntropy.gradient(ctx, go, *saved)
+            grad = _NoSecondDerivative.apply(grad, saved[0], go)
+        else:
+            grad = _CrossEntropy.gradient(ctx, go, *saved)
+        return (grad,) + (None,) * 8
+
+    @staticmethod
+    def gradient(ctx, go, logits, targets, weight, legal):
         grad = ctx.ready
         ctx.ready = None                       # handed out once; a second backward pass gets memory of its own
         skip = grad is not None
@@ -119,12 +125,15 @@ class _CrossEntropy(torch.autograd.Function):
                 go = go.contiguous()
             ws = torch.empty(nbytes, dtype=torch.uint8, device=grad.device)   # not the forward's: a captured backward keeps its own
             L.call_on(grad.get_device(), "mz_policy_loss", _LOSS_ARGS(*head, go.data_ptr(), 0, 0, grad.data_ptr(), *sizes, *strides, *rest, go.dim(), skip), ws.data_ptr(), nbytes)
-        return (grad,) + (None,) * 9
+        return grad
 
 
 class _NoSecondDerivative(torch.autograd.Function):
+    """The gradient as a function of the logits and of the loss's own gradient: whatever is asked for behind either of them, a backward pass
+    that would need this one's derivative comes through here."""
+
     @staticmethod
-    def forward(ctx, grad):
+    def forward(ctx, grad, logits, go):
         return grad.view_as(grad)
 
     @staticmethod
