@@ -8,7 +8,7 @@
 // actions on it": nothing is sorted.
 //
 // All masses are held in 64 bits, because a draw next to the border of two actions has to fall on its own side: at 131,072 actions f32 sums would put
-// one draw in a thousand wrong.  Sums run in a fixed order, or over integers (w scaled to 2^s, so that atomics give the same total in any order).
+// one draw in a thousand wrong.  Sums run in a fixed order, or over integers (units of the total's 2^61st part, so that atomics give the same total in any order).
 //
 // Up to 512 actions: one wave per row.  Up to 8192: one workgroup of 4, 8 or 16 waves per row.  Both hold the row in registers, one launch; they are
 // bound by latency (4096 x 65 f32 4.5 us, 256 x 4096 f32 top-p 9 us).
@@ -496,11 +496,13 @@ __device__ __forceinline__ bool find_threshold(EACH each, uint32_t lo, uint32_t 
     }
 }
 
-// masses as integers: at most 2^50 each, their sum over v actions below 2^63
-__device__ __forceinline__ double int_scale(int v) { return ldexp(1.0, min(50, 62 - (32 - __clz(v)))); }
-__device__ __forceinline__ uint64_t int_mass(double w, double scale) {   // the mantissa of w scale + 2^52 holds it, rounded
-    return (uint64_t)__double_as_longlong(fma(w, scale, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
-}
+// Masses as integers, for sums that the order of atomics does not change: the total that is shared out becomes 2^61 .. 2^62, so a unit is 2^-61 of it at
+// most and 2^19 masses, each rounded by half a unit, are 2^-43 of it off together: as far as a 64-bit sum of them in one chain.  (In units of the BEST
+// mass, 2^-44 of it, a long tail behind one action far ahead was cut a fifth too short.)
+__device__ __forceinline__ double int_scale(double total) { return ldexp(1.0, 61 - ilogb(total)); }
+__device__ __forceinline__ uint64_t int_mass(double w, double scale) { return (uint64_t)fma(w, scale, 0.5); }
+// how many of up to `ties` actions of mass w begin before `left` is used up
+__device__ __forceinline__ uint32_t ties_within(double left, double w, uint32_t ties) { return left > 0.0 ? (uint32_t)fmin(ceil(left / w), (double)ties) : 0; }
 
 // The answer for what the workgroup's threads hold in registers, thread by thread in the actions' order, N in each: the place of the picked one
 // (thread N + j), in every thread.  best: the largest key.  low: nothing below it is kept.  all: the mass that top-p shares out, if it is known (> 0).
@@ -536,35 +538,29 @@ __device__ __forceinline__ int pick(const float *x, const Setting &s, double u, 
             }
         }
         if (s.p_on) {
-            const uint32_t lowest = tau > KEY_NONE ? tau : low;
-            const double scale = int_scale(v);
-            double limit;
-            if (all > 0.0) limit = s.top_p * all * scale;
-            else {
-                uint64_t sum = 0;
+            // The cut is looked for above top-k's threshold (on it lie more actions than top-k keeps); where those above do not fill p, on it.
+            double over = 0.0;
+            const double wt = tau > KEY_NONE ? mass_of(value_of(tau), m, s.c) : 0.0;
+            if (!(all > 0.0)) {
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const uint32_t key = key_of(x[j]);
-                    if (key > tau && key >= lowest) sum += int_mass(w[j], scale);
-                }
-                sum = block_total<W>(sum, (uint64_t *)S.wave_u64);
-                if (tau > KEY_NONE) sum += ties * int_mass(mass_of(value_of(tau), m, s.c), scale);
-                limit = s.top_p * (double)sum;
+                for (int j = 0; j < N; ++j) over += key_of(x[j]) > tau ? w[j] : 0.0;
+                over = block_total<W>(over, S.wave_f64);
+                all = over + ties * wt;
             }
-            const uint64_t amount = (uint64_t)fmax(1.0, ceil(limit));
+            const uint32_t from = tau > KEY_NONE ? tau + 1 : low;
+            const double scale = int_scale(all);
+            const uint64_t amount = (uint64_t)fmax(1.0, ceil(s.top_p * all * scale));
             auto each = [&](auto take) {
+                double by = scale;
+                asm volatile("" : "+v"(by));     // not the same value to the compiler, which would keep all integers beside the masses
 #pragma unroll
-                for (int j = 0; j < N; ++j) take(key_of(x[j]), x[j], [&] { return int_mass(w[j], scale); });
+                for (int j = 0; j < N; ++j) take(key_of(x[j]), x[j], [&] { return int_mass(w[j], by); });
             };
             uint32_t t;
-            if (find_threshold(each, lowest, lowest, best, amount, ENDS, S, &t, &above)) {
-                const uint64_t one = max((uint64_t)1, int_mass(mass_of(value_of(t), m, s.c), scale));
-                const uint32_t r = (uint32_t)min((amount - above + one - 1) / one, (uint64_t)v);
-                if (t > tau) {
-                    tau = t;
-                    ties = r;
-                } else ties = min(ties, r);
-            }
+            if (from <= best && find_threshold(each, from, from, best, amount, ENDS, S, &t, &above)) {
+                ties = ties_within((double)(amount - above), mass_of(value_of(t), m, s.c) * scale, v);
+                tau = t;
+            } else if (tau > KEY_NONE) ties = max(tau == best ? 1u : 0u, ties_within(s.top_p * all - over, wt, ties));
         }
     }
     // cumulated in the actions' order
@@ -971,8 +967,6 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
             }
 
             // Too many for the registers: the same steps with the row read again for each.
-            const double scale = int_scale(A.v);
-            auto mass_int = [&](float x) { return int_mass(mass_of(x, m, s.c), scale); };
             uint64_t above;
             if (s.k) {
                 uint32_t t;
@@ -989,41 +983,34 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
                 }
             }
             if (s.p_on) {
-                const uint32_t lowest = tau > KEY_NONE ? tau : low;
-                listed = list_groups(lowest);
-                double limit;
-                if (massed) limit = s.top_p * all * scale;
-                else {
-                    uint64_t sum = 0;
+                const uint32_t from = tau > KEY_NONE ? tau + 1 : low;   // as in `pick`
+                double over = 0.0;
+                const double wt = tau > KEY_NONE ? mass_of(value_of(tau), m, s.c) : 0.0;
+                listed = list_groups(from);
+                if (!massed) {
                     walk(listed, [&](int, const float *x) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const uint32_t key = key_of(x[j]);
-                            if (key > tau && key >= lowest) sum += mass_int(x[j]);
-                        }
+                        for (int j = 0; j < 8; ++j)
+                            if (key_of(x[j]) >= from) over += mass_of(x[j], m, s.c);
                         return true;
                     });
-                    sum = block_total<W>(sum, (uint64_t *)S.wave_u64);
-                    if (tau > KEY_NONE) sum += ties * mass_int(value_of(tau));
-                    limit = s.top_p * (double)sum;
+                    over = block_total<W>(over, S.wave_f64);
                 }
-                const uint64_t amount = (uint64_t)fmax(1.0, ceil(limit));
+                const double shared = massed ? all : over + ties * wt, scale = int_scale(shared);
+                const uint64_t amount = (uint64_t)fmax(1.0, ceil(s.top_p * shared * scale));
                 uint32_t t;
                 auto each = [&](auto take) {
                     walk(listed, [&](int, const float *x) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) take(key_of(x[j]), x[j], [&] { return mass_int(x[j]); });
+                        for (int j = 0; j < 8; ++j) take(key_of(x[j]), x[j], [&] { return int_mass(mass_of(x[j], m, s.c), scale); });
                         return true;
                     });
                 };
-                if (find_threshold(each, lowest, lowest, best, amount, ENDS, S, &t, &above)) {
-                    const uint64_t one = max((uint64_t)1, mass_int(value_of(t)));
-                    const uint32_t r = (uint32_t)min((amount - above + one - 1) / one, (uint64_t)A.v);
-                    if (t > tau) {
-                        tau = t;
-                        ties = r;
-                    } else ties = min(ties, r);
-                } else if (tau <= KEY_NONE) tau = low - 1;   // rounding: everything from `low` on
+                if (from <= best && find_threshold(each, from, from, best, amount, ENDS, S, &t, &above)) {
+                    ties = ties_within((double)(amount - above), mass_of(value_of(t), m, s.c) * scale, A.v);
+                    tau = t;
+                } else if (tau > KEY_NONE) ties = max(tau == best ? 1u : 0u, ties_within(s.top_p * shared - over, wt, ties));
+                else tau = low - 1;   // rounding: everything from `low` on
             }
             // what is kept of every group, and how many actions on the threshold come before it
             uint32_t on = 0;
