@@ -51,13 +51,14 @@ __device__ __forceinline__ Setting setting_of(const SampleArgs &A, int64_t row) 
     const double T = A.temperature_of ? (double)A.temperature_of[row] : A.temperature;
     s.bad = !(T < INFINITY);
     s.top_p = fmax(A.top_p_of ? (double)A.top_p_of[row] : A.top_p, 0.0);
-    s.min_p = A.min_p_of ? (double)A.min_p_of[row] : A.min_p;
+    const double min_p = A.min_p_of ? (double)A.min_p_of[row] : A.min_p;
+    s.min_p = fmin(min_p, 1.0);
     const int k = A.top_k_of ? A.top_k_of[row] : A.top_k;
     s.k = k > 0 && k < A.v ? k : 0;
     s.greedy = !(T > 0.0) || s.k == 1;
     s.c = s.greedy ? 0.0 : A.temperature_of ? 1.4426950408889634 / T : A.c;
     s.p_on = (A.top_p_of ? (double)A.top_p_of[row] : A.top_p) < 1.0;   // a NaN is no limit
-    s.m_on = s.min_p > 0.0;
+    s.m_on = min_p > 0.0;
     return s;
 }
 
@@ -758,7 +759,8 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
                 const float f = (float)(x - 1e-6 * (fabs(x) + fabs(m)));
                 return max(low, min(best, max(key_of(f), KEY_LOWEST + 2) - 2));
             };
-            if (s.m_on && !(s.k && s.p_on)) low = bound(m + log2(fmin(s.min_p, 1.0)) / s.c);
+            // (1e-12: w rounds up to min_p at that distance too, and at a high temperature a step of w is far in x.)
+            if (s.m_on && !(s.k && s.p_on)) low = bound(m + (log2(s.min_p) - 1e-12) / s.c);
             if (s.k) {                           // each wave takes every W-th group: if q = k / W of them reach a value in every wave, k actions do
                 const int q = (s.k + W - 1) / W;
                 uint32_t t = 0;
