@@ -2,9 +2,12 @@
 loss.backward() and optimizer.step() (main.py:266-267) when a step must not be allowed to run away.
 
 A list of tensors is one operator: one launch per 256 tensors for the norm and per 128 for the scaling, whatever their sizes; the flat
-buffer of a ``train.FlatGradBucket`` is a list of one.  Nothing here waits for the GPU.  No CPU fallback: host tensors raise."""
-import array
+buffer of a ``train.FlatGradBucket`` is a list of one.  Nothing here waits for the GPU.  No CPU fallback: host tensors raise.
+
+Neither has a derivative: where tensors carry a graph of their own and gradients are recorded, a backward pass that comes to the norm
+or to what was scaled raises an error (not under torch.no_grad(), nor for leaves, which are scaled as values, as an optimiser does)."""
 import operator
+import struct
 
 import torch
 
@@ -49,26 +52,59 @@ def _columns(who, tensors):
     return list(map(_T.data_ptr, tensors)), list(map(_T.numel, tensors)), codes, index, together
 
 
-def _call(name, dev, table_columns, index, *args):
-    k = len(table_columns[0])
+class _NoDerivative(torch.autograd.Function):
+    """the norm as a function of the tensors"""
+
+    @staticmethod
+    def forward(ctx, norm, *tensors):
+        return norm.view_as(norm)
+
+    @staticmethod
+    def backward(ctx, go):
+        raise L.MzError("gradnorm: the norm and the clipping have no derivative (detach the tensors, or call under torch.no_grad())")
+
+
+class _ScaledInPlace(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tensor):
+        ctx.mark_dirty(tensor)
+        return tensor
+
+    backward = _NoDerivative.backward
+
+
+def _recorded(tensors):
+    """those that carry a graph, where gradients are recorded.  (One pass over the list in torch itself.)"""
+    if torch.is_grad_enabled() and torch._C._any_requires_grad(*tensors):
+        return [t for t in tensors if t.requires_grad]
+    return []
+
+
+def _call(name, dev, src, dst, sizes, types, index, *args):
+    k = len(src)
     words = [0] * (4 * k)                      # mz_grad_tensor: src, dst, n, src_dtype | dst_dtype << 32
-    for c in range(4):
-        words[c::4] = table_columns[c]
-    table = array.array("q", words)
+    words[::4] = src
+    if dst is not None:
+        words[1::4] = dst
+    words[2::4] = sizes
+    words[3::4] = types
+    table = struct.pack("%dq" % (4 * k), *words)
     nbytes = L.lib.mz_grad_workspace_bytes(k)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    L.call_on(index, name, table.buffer_info()[0], k, *args, ws.data_ptr(), nbytes, norm.data_ptr())
+    L.call_on(index, name, table, k, *args, ws.data_ptr(), nbytes, norm.data_ptr())
     return norm
 
 
 def grad_norm(tensors):
     """sqrt of the sum of squares over all elements of `tensors` (a tensor or a list; float32 / bfloat16 / float16, mixed as they come,
-    elements lying together in any order of the axes) as a 0-d float32 tensor.  The sums are held in 64 bits in a fixed order.
+    elements lying together in any order of the axes) as a 0-d float32 tensor without a derivative.  The sums are held in 64 bits in a fixed order.
     inf or NaN among the elements gives inf or NaN."""
     tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
     ptrs, sizes, codes, index, _ = _columns("grad_norm", tensors)
-    return _call("mz_grad_norm", tensors[0].device, (ptrs, ptrs, sizes, codes), index)
+    norm = _call("mz_grad_norm", tensors[0].device, ptrs, None, sizes, codes, index)
+    recorded = _recorded(tensors)
+    return _NoDerivative.apply(norm, *recorded) if recorded else norm
 
 
 def clip_grad_norm(tensors, max_norm, out=None):
@@ -94,7 +130,16 @@ def clip_grad_norm(tensors, max_norm, out=None):
             raise L.MzError("%s: out has to have the gradients' shapes and strides" % who)
         if dst_codes != codes and any(d != s and d != L.MZ_F32 for s, d in zip(codes, dst_codes)):
             raise L.MzError("%s: out has the gradients' dtype or float32" % who)
-    types = [s | d << 32 for s, d in zip(codes, dst_codes)]
-    norm = _call("mz_grad_clip", tensors[0].device, (ptrs, dst, sizes, types), index, max_norm)
+    recorded = _recorded(tensors)
+    if recorded and out is not None:
+        raise L.MzError("%s: out= takes no tensors that carry a graph (detach them, or call under torch.no_grad())" % who)
+    inner = [t for t in (recorded if out is None else _recorded(outs)) if not t.is_leaf]
+    for t in inner:
+        _ScaledInPlace.apply(t)
+    if out is None and codes.count(codes[0]) == len(codes):
+        types = [codes[0] * (1 + (1 << 32))] * len(codes)
+    else:
+        types = [s | d << 32 for s, d in zip(codes, dst_codes)]
+    norm = _call("mz_grad_clip", tensors[0].device, ptrs, dst, sizes, types, index, max_norm)
     torch.autograd.graph.increment_version(outs)      # autograd's check of tensors changed in place sees these too
-    return norm
+    return _NoDerivative.apply(norm, *inner) if inner else norm
