@@ -53,6 +53,8 @@ extern "C" {
 
 const char *mz_last_error(void);
 int mz_version(void);
+/* id (host memory): which capture into a graph `stream` is in, another number for each; 0 = none */
+int mz_capture_id(void *stream, uint64_t *id);
 
 /* ------------------------------------------------------------------------------------------
  * Environment (reversi.py:39-205)

@@ -133,6 +133,7 @@ SIGNATURES = {
     "mz_restower_x3_stamps": [_p, _p, _p, _p, _i64, _p, _p],
     "mz_tower_x3_pack_ends": [_p, _i32, _p, _p, _p],
     "mz_tower_x3_forward": [_p, _p, _p, _p, _p, _i32, _p, _p, _i64, _p],
+    "mz_capture_id": [_p, C.POINTER(C.c_uint64)],
     "mz_sample_actions": [_p, _p, _i64, _p],   # SampleArgs, or its bytes
     "mz_policy_loss": [_p, _p, _i64, _p],      # PolicyLossArgs, or its bytes
     "mz_grad_norm": [_p, _i32, _p, _i64, _p, _p],
@@ -175,6 +176,18 @@ def call_on(index, name, *args):
     rc = getattr(lib, name)(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc != 0:
         raise MzError("%s failed (%d): %s" % (name, rc, lib.mz_last_error().decode()))
+
+
+def capture_id(index):
+    """which capture into a graph the current stream of GPU `index` is in; 0 = none"""
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return capture_id(index)
+    if not torch._C._cuda_isCurrentStreamCapturing():
+        return 0
+    out = C.c_uint64()
+    call("mz_capture_id", torch._C._cuda_getCurrentRawStream(index), C.byref(out))
+    return out.value
 
 
 def current_stream():

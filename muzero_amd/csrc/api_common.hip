@@ -13,3 +13,12 @@ void mz_set_error(const char *fmt, ...) {
 
 extern "C" const char *mz_last_error(void) { return g_err; }
 extern "C" int mz_version(void) { return 1; }
+
+extern "C" int mz_capture_id(void *stream, uint64_t *id) {
+    MZ_REQUIRE(id, "mz_capture_id: null id");
+    hipStreamCaptureStatus status;
+    unsigned long long n = 0;
+    MZ_HIP(hipStreamGetCaptureInfo((hipStream_t)stream, &status, &n));
+    *id = status == hipStreamCaptureStatusNone ? 0 : (uint64_t)n + 1;
+    return MZ_OK;
+}

@@ -86,6 +86,7 @@ class _CrossEntropy(torch.autograd.Function):
             ctx.call = head, sizes, strides, rest, nbytes
             if reduction != "none":
                 grad = torch.empty((n, v), dtype=logits.dtype, device=dev)
+                ctx.capture = L.capture_id(dev.index)
             ctx.ready = grad
         if n == 0:
             return out.fill_(float("nan") if reduction == "mean" else 0.0)
@@ -110,8 +111,10 @@ class _CrossEntropy(torch.autograd.Function):
     def gradient(ctx, go, logits, targets, weight, legal):
         grad = ctx.ready
         ctx.ready = None                       # handed out once; a second backward pass gets memory of its own
-        skip = grad is not None
-        if grad is None:
+        # ... and so does one in another capture than its forward pass: it may replay without that, and once another factor was there the memory holds
+        # that one's gradient.
+        skip = grad is not None and ctx.capture == L.capture_id(grad.get_device())
+        if not skip:
             grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         if logits.shape[0]:
             head, sizes, strides, rest, nbytes = ctx.call

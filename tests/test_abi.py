@@ -66,3 +66,9 @@ def test_host_tensors_are_refused():
     from muzero_amd import _lib as L
     with pytest.raises(L.MzError):
         L.dptr(torch.zeros(4))
+
+
+def test_a_capture_needs_a_place_for_its_number():
+    from muzero_amd import _lib as L
+    with pytest.raises(L.MzError, match="null id"):
+        L.call("mz_capture_id", None, None)
