@@ -20,6 +20,7 @@ from .selfplay import SelfPlayEngine
 
 NUM_SIMULATIONS = 100   # test.py:143
 TEMPERATURE = 0.25      # test.py:174
+PASS = 64
 
 
 def controller_image(hist_white, hist_black, state_index, n, dtype=torch.float32, out=None):
@@ -49,7 +50,8 @@ def play_games(black_net, white_net, n_games, num_simulations=NUM_SIMULATIONS, t
     """n_games lock-step games, `black_net` moving for BLACK and `white_net` for WHITE (the loop of
     test.py:45-65).  Networks follow the engine protocol (InferenceEngine / NetworkAdapter).
     num_simulations=0: no search, every move straight from the mover's policy over its legal moves (policy.sample_actions at the same
-    temperature) -- what the networks know without the tree.
+    temperature) -- what the networks know without the tree.  From its logits, where the network has policy_logits(hidden); from
+    the probabilities otherwise, where those below 1.2e-38 count as that much (so legal moves without any are equally likely).
     u: optional (steps, n) float64 uniforms for the sampled moves.  Returns ArenaResult with actions
     (steps, n) uint8 and the final disc counts (test.py:67-68)."""
     n, T = int(n_games), int(max_steps if max_steps is not None else config.max_moves)
@@ -77,8 +79,10 @@ def play_games(black_net, white_net, n_games, num_simulations=NUM_SIMULATIONS, t
             visits, _ = eng.search(image, noise=None)   # expand_node + run_mcts, no add_exploration_noise (test.py:37-41)
             a = softmax_sample(visits, temperature, ut)
         else:
-            probs = net.initial(controller_image(hw, hb, t, n, getattr(net, "dtype", torch.float32)))[1]
-            a = sample_actions(probs.float().log(), ut, temperature, legal=env.legal).to(torch.uint8)   # -1 (a policy without mass) is refused as a move
+            _, probs, hidden = net.initial(controller_image(hw, hb, t, n, getattr(net, "dtype", torch.float32)))
+            logits = net.policy_logits(hidden) if hasattr(net, "policy_logits") else probs.float().clamp(min=torch.finfo(torch.float32).tiny).log()
+            a = sample_actions(logits, ut, temperature, legal=env.legal)
+            a = a.masked_fill(env.done != 0, PASS).to(torch.uint8)   # -1 (a NaN among the logits) is refused as a move; a finished game makes none
         _, status = env.step(a)   # finished games report MZ_ST_DONE and stay untouched
         bad |= status == L.ST_ILLEGAL
         actions[t].copy_(a)

@@ -89,6 +89,16 @@ class Prediction(nn.Module):
         return self.policy_head(x), self.value_head(x)
 
 
+@torch.no_grad()
+def policy_logits(prediction, hidden):
+    """(n, 65) float32: what the policy head takes the softmax of, from hidden states of any type, in float32 whatever the weights'
+    type (the 1x1 convolution as a matrix product).  A probability underflows where a logit does not."""
+    ph = prediction.policy_head
+    f = lambda t: t.detach().float()  # noqa: E731
+    x = torch.relu(f(ph[0].weight).flatten(1) @ hidden.float().flatten(2) + f(ph[0].bias).unsqueeze(1)).flatten(1)
+    return F.linear(torch.relu(F.linear(x, f(ph[3].weight), f(ph[3].bias))), f(ph[5].weight), f(ph[5].bias))
+
+
 class Network(nn.Module):
     """network.py:137-167"""
 
@@ -440,6 +450,10 @@ class InferenceEngine:
         if self.tower == "hip_x3":
             return self._infer_x3("repr", image.to(self.dtype))
         return self._finish(self._hidden_initial(image.to(self.dtype)))
+
+    def policy_logits(self, hidden):
+        """the logits behind the policy that initial() / recurrent() returned together with `hidden`"""
+        return policy_logits(self.net.prediction, hidden)
 
     @torch.no_grad()
     def recurrent(self, x10, out=None):
