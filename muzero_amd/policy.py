@@ -72,10 +72,9 @@ class _CrossEntropy(torch.autograd.Function):
     computes the rows again, so a scaled 16-bit gradient is rounded once, after the scale."""
 
     @staticmethod
-    def forward(ctx, logits, targets, weight, legal, reduction, head, sizes, strides, rest):
+    def forward(ctx, logits, targets, weight, legal, reduction, head, sizes, strides, rest, need):
         n, v = logits.shape
         dev = logits.device
-        need = ctx.needs_input_grad[0]
         out = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32, device=dev)
         nbytes = L.lib.mz_policy_loss_workspace_bytes(n, v)
         if nbytes < 0:
@@ -105,7 +104,7 @@ class _CrossEntropy(torch.autograd.Function):
             grad = _NoSecondDerivative.apply(grad, saved[0], go)
         else:
             grad = _CrossEntropy.gradient(ctx, go, *saved)
-        return (grad,) + (None,) * 8
+        return (grad,) + (None,) * 9
 
     @staticmethod
     def gradient(ctx, go, logits, targets, weight, legal):
@@ -160,7 +159,8 @@ def cross_entropy(logits, targets, weight=None, legal=None, reduction="mean"):
         raise L.MzError("%s: reduction is 'mean', 'sum' or 'none', got %r" % (who, reduction))
     n, v = logits.shape
     rest = v, 1.0 / n if reduction == "mean" and n else 1.0, _DT[logits.dtype], _DT[targets.dtype]
-    return _CrossEntropy.apply(logits, targets, weight, legal, reduction, head, (n, v), strides, rest)
+    need = logits.requires_grad and torch.is_grad_enabled()   # asked for here: inside forward, gradients are never recorded
+    return _CrossEntropy.apply(logits, targets, weight, legal, reduction, head, (n, v), strides, rest, need)
 
 
 def _setting(who, name, value, n, dtype, dev, low, high):
