@@ -333,7 +333,8 @@ def update_weights(optimizer, network, batch, bucket=None, group=None, amp_dtype
     kernels; implies batched.  "x3": the same kernels in split precision (every fp32 product as three bf16 MFMA products: close to
     fp32, tests/test_gpu_train.py holds it to the reference's recorded gradients).  False = the reference's fp32 arithmetic.
     max_grad_norm: scale the (averaged) gradients to a 2-norm of at most this before the step (gradnorm.clip_grad_norm); None = the
-    reference's step, which has no such guard.  policy_from_logits: see muzero_loss_batched; implies batched.  Both need the GPU."""
+    reference's step, which has no such guard.  The norm they had is network.grad_norm then, a 0-d tensor that is not waited for.  Clipping
+    bounds finite gradients only: where the norm is inf or NaN the step is taken all the same, with what the formula gives.  policy_from_logits: see muzero_loss_batched; implies batched.  Both need the GPU."""
     if (max_grad_norm is not None or policy_from_logits) and not next(network.parameters()).is_cuda:
         raise RuntimeError("update_weights(max_grad_norm=, policy_from_logits=) needs the network on a GPU: the kernels have no CPU fallback")
     if policy_from_logits and amp_dtype is not None:
@@ -374,10 +375,10 @@ def update_weights(optimizer, network, batch, bucket=None, group=None, amp_dtype
         raise RuntimeError("data-parallel update_weights needs a FlatGradBucket")
     if max_grad_norm is not None:      # behind the all-reduce: every rank scales the same gradients by the same factor
         if bucket is not None:
-            bucket.clip(max_grad_norm)
+            network.grad_norm = bucket.clip(max_grad_norm)
         else:
             from .gradnorm import clip_grad_norm
-            clip_grad_norm([p.grad for p in network.parameters() if p.grad is not None], max_grad_norm)
+            network.grad_norm = clip_grad_norm([p.grad for p in network.parameters() if p.grad is not None], max_grad_norm)
     optimizer.step()
     if LOG is not None and network.steps % 10 == 0:   # main.py:268-269; the float() is a device sync
         LOG('step {}: p_loss {:.4f} v_loss {:.4f}'.format(network.steps, float(p_loss.detach()), float(v_loss.detach())))
