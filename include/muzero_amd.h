@@ -547,7 +547,8 @@ int mz_grad_clip(const mz_grad_tensor *tensors, int32_t count, double max_norm, 
  *     grad_i = grad_out w_i scale (T exp(x - m) / z - t), 0 where not legal
  * A term with t = 0 counts as 0 also where x = -inf.  A row without a legal action above -inf, or with w_i = 0, gives loss 0 and
  * gradient 0 whatever it holds; values at places that are not legal are never used.  NaN and +inf elsewhere make their row NaN.
- * Softmax and row sums in f32, the sum over rows in 64 bits in a fixed order, gradients rounded once to the logits' dtype. */
+ * Softmax and row sums in f32 (16-bit logits above 512 actions: exponentials to |x - m| 2^-24 of themselves), the sum over rows in 64 bits in a
+ * fixed order, gradients rounded once to the logits' dtype. */
 typedef struct mz_policy_loss_args {
     const void *logits;         /* (n, v) of dtype, rows logits_stride elements apart */
     const void *targets;        /* (n, v) of target_dtype (dtype, or MZ_F32), rows targets_stride apart */
@@ -579,8 +580,9 @@ int mz_policy_loss(const mz_policy_loss_args *args, void *workspace, int64_t wor
  *     min_p > 0       : of these, the ones with w_j >= min_p
  *     the first of the order always stays; with R the mass of what stays, the answer is the lowest index j with
  *     sum over kept i <= j of w_i > u R   (the last kept action if rounding, or u >= 1, leaves none).
- * Masses in 64 bits, in an order that does not change between calls.  A row without a legal action above -inf, with a NaN or +inf
- * at a legal place, or with a NaN or infinite temperature answers -1.  Values at places that are not legal are never used. */
+ * Masses in 64 bits, in an order that does not change between calls; above 8192 actions (4096 with more than 512 rows) the total of a row comes from masses
+ * of 128 actions that are right to 2e-12.  A row without a legal action above -inf, with a NaN or +inf at a legal place, or with a temperature of NaN
+ * or +inf answers -1.  Values at places that are not legal are never used. */
 typedef struct mz_sample_args {
     const void *logits;             /* (n, v) of dtype, rows logits_stride elements apart */
     const uint8_t *allowed;         /* (n, v) bytes, 0 = not legal, rows allowed_stride apart; NULL = all legal */

@@ -10,7 +10,8 @@
 // 4096 x 32768 bf16 takes 155 us, 5.2 TB/s, where a large copy reaches 4.7.  Rows that are too long for a workgroup's registers are cut into chunks:
 // one launch for the chunks' sums, one that joins them and writes the gradient (both read x and t: 5 parts of traffic for 3; in slabs of rows that
 // would stay in the last-level cache between the two launches it was slower, 512 x 131072 f32: 310 us in slabs of 96 MB, 263 us without).
-// Softmax statistics and row sums are f32, sums over rows 64 bits; 16-bit gradients are rounded once.
+// Softmax statistics and row sums are f32, sums over rows 64 bits; 16-bit gradients are rounded once.  Above 512 actions the exponentials of 16-bit
+// logits are the hardware's, also those in the f32 loss (exp_of).
 #include <math.h>
 #include <algorithm>
 #include "numeric.h"

@@ -8,10 +8,12 @@
 // actions on it": nothing is sorted.
 //
 // All masses are held in 64 bits, because a draw next to the border of two actions has to fall on its own side: at 131,072 actions f32 sums would put
-// one draw in a thousand wrong.  Sums run in a fixed order, or over integers (units of the total's 2^61st part, so that atomics give the same total in any order).
+// one draw in a thousand wrong.  Sums run in a fixed order, or over integers (units of the total's 2^61st part, so that atomics give the same total in any
+// order).  The groups' masses of long rows are right to 2e-12.
 //
-// Up to 512 actions: one wave per row.  Up to 8192: one workgroup of 4, 8 or 16 waves per row.  Both hold the row in registers, one launch; they are
-// bound by latency (4096 x 65 f32 4.5 us, 256 x 4096 f32 top-p 9 us).
+// Up to 512 actions: one wave per row.  Up to 8192: one workgroup of 4, 8 or 16 waves per row.  Both hold the row in registers, one launch; few rows are
+// bound by latency (4096 x 65 f32 without a filter 4.3 us, 256 x 4096 bf16 top-p 9 us), thousands under top-p by the search for its cut (4096 x 500 f32
+// 27 us, 4096 x 4096 bf16 75 us, over ten times what reading them takes): a 64-bit exponential for every action, and above 512 of them an LDS atomic.
 // Longer rows, two launches: k_sample_groups reads the logits once, across all CUs, and leaves the maximum of every 128 actions and, where the
 // row's settings need the total, their mass (256 x 131072 bf16: without the masses 13 us, the memory's time; with them 30 us, the 64-bit exponentials', which
 // keep the vector ALUs 70 % busy).  k_sample_row, a workgroup per row, works from those: bounds on what can be kept leave few groups, it reads only these
@@ -409,7 +411,7 @@ template <int W> __device__ __forceinline__ int crossing_bin(Shared<W> &S, uint6
 // not matter.  `guess` >= lo: where tau is looked for first; `ends` = bits of a key that its type leaves empty.
 // The first histogram, from `guess` on, has bins of equal width in the value, which few logits share; the up to 64 of the bin that reaches the limit
 // are ranked in registers.  More: histograms over the bits of that bin's keys, each narrowing to one bin of the one before, unless they are all equal
-// (256 x 131072 bf16, flat, p = 0.9: 189 us; from all keys 259).  Tau below the guess: the same from all keys.
+// (256 x 131072 bf16, flat, p = 0.9: 190 us; from all keys 259).  Tau below the guess: the same from all keys.
 template <int W, class EACH>
 __device__ __forceinline__ bool find_threshold(EACH each, uint32_t lo, uint32_t guess, uint32_t hi, uint64_t limit, int ends, Shared<W> &S,
                                                uint32_t *tau, uint64_t *above_out) {
@@ -498,8 +500,8 @@ __device__ __forceinline__ bool find_threshold(EACH each, uint32_t lo, uint32_t 
 }
 
 // Masses as integers, for sums that the order of atomics does not change: the total that is shared out becomes 2^61 .. 2^62, so a unit is 2^-61 of it at
-// most and 2^19 masses, each rounded by half a unit, are 2^-43 of it off together: as far as a 64-bit sum of them in one chain.  (In units of the BEST
-// mass, 2^-44 of it, a long tail behind one action far ahead was cut a fifth too short.)
+// most and 2^19 masses, each rounded by half a unit, are 2^-43 of it off together.  (In units of 2^-44 of the BEST mass a long tail behind one action
+// far ahead would be cut a fifth too short.)
 __device__ __forceinline__ double int_scale(double total) { return ldexp(1.0, 61 - ilogb(total)); }
 __device__ __forceinline__ uint64_t int_mass(double w, double scale) { return (uint64_t)fma(w, scale, 0.5); }
 // how many of up to `ties` actions of mass w begin before `left` is used up
@@ -1135,8 +1137,8 @@ template <int XD, int W, int N> __global__ void __launch_bounds__(64 * W) k_samp
 
 template <int XD> int launch(const SampleArgs &A, void *workspace, hipStream_t s) {
     const unsigned rows = (unsigned)A.n;
-    // top-p, 4096 x 500 f32: a wave a row 26.5 us, a workgroup 33.7.  4096 x 2000 f32: four waves a row 35.6 us, eight 75.6.  4096 x 4096 bf16: in one
-    // launch 74 us, in two 98.  8192 f32: 256 rows 14.0 and 24.1 us, 2048 rows 98 and 77.
+    // top-p, 4096 x 500 f32: a wave a row 26.6 us, a workgroup 32.6.  4096 x 2000 f32: four waves a row 34.1 us, eight 72.6.  4096 x 4096 bf16: in one
+    // launch 75 us, in two 100.  8192 f32: 256 rows 13.3 and 21.7 us, 2048 rows 97 and 76.
     if (A.v <= 128) hipLaunchKernelGGL((k_sample_wave<XD, 2>), dim3((rows + 3) / 4), dim3(256), 0, s, A);
     else if (A.v <= 512) hipLaunchKernelGGL((k_sample_wave<XD, 8>), dim3((rows + 3) / 4), dim3(256), 0, s, A);
     else if (A.v <= 2048) hipLaunchKernelGGL((k_sample_block<XD, 4>), dim3(rows), dim3(256), 0, s, A);
@@ -1168,7 +1170,7 @@ template <int XD> int launch(const SampleArgs &A, void *workspace, hipStream_t s
                 hipLaunchKernelGGL((k_sample_groups<XD, 1>), dim3((A.v + 2047) / 2048, (unsigned)B.n), dim3(256), 0, s, B, groups, row_mass, row_top);
             MZ_LAUNCH_CHECK("k_sample_groups");
             // up to a row per CU: sixteen waves each; more rows: eight waves each, so that a CU works on two (131,072 bf16, sixteen / eight: 256 rows top-p
-            // 54 / 54 us, top-k 1000 88 / 123 us; 400 rows top-p 90 / 82 us, top-k 50 43 / 35 us)
+            // 54 / 57 us, top-k 1000 68 / 95 us; 400 rows top-p 84 / 73 us, top-k 50 44 / 36 us)
             const size_t lds = (size_t)groups * 12;
             const double *m = row_mass;
             const uint32_t *t = row_top;

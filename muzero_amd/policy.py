@@ -69,7 +69,8 @@ def _places(who, logits, targets, weight, legal):
 class _CrossEntropy(torch.autograd.Function):
     """The gradient comes out of the forward pass over the rows, for a loss whose own gradient is 1 (what loss.backward() starts
     from).  backward launches the same kernel with the gradient it is given: where that is 1 the kernel leaves at once, otherwise it
-    computes the rows again, so a scaled 16-bit gradient is rounded once, after the scale."""
+    computes the rows again, so a scaled 16-bit gradient is rounded once, after the scale.  No gradient comes out of the forward pass where
+    none is recorded, or where each row has a factor of its own ("none")."""
 
     @staticmethod
     def forward(ctx, logits, targets, weight, legal, reduction, head, sizes, strides, rest, need):
@@ -179,10 +180,11 @@ def sample_actions(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, le
     fewest most likely that together reach the share top_p, of these to the ones at least min_p times as likely as the best; equal
     logits go to the lower index, the best action always stays, temperature 0 takes it.  The answer is the lowest index at which the
     kept mass, cumulated in the order of the indices, exceeds u times its total.  Every setting is a number, or a tensor with one value
-    per row (float32; top_k int32).  Masses are held in 64 bits in a fixed order: the same call gives the same actions.
+    per row (float32; top_k int32).  Masses are held in 64 bits in a fixed order (a long row's total comes from masses of 128
+    actions that are right to 2e-12): the same call gives the same actions.
 
     logits float32 / bfloat16 / float16, up to 2^19 actions, rows may be strided; legal: see the module.  A row without a legal action
-    (all others -inf count as not legal), with NaN or +inf at a legal place, or with a NaN or infinite temperature gives -1.  out: int32
+    (all others -inf count as not legal), with NaN or +inf at a legal place, or with a temperature of NaN or +inf gives -1.  out: int32
     (n,) to write into."""
     who = "sample_actions"
     stride = _rows(who, "logits", logits)
