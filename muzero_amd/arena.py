@@ -79,8 +79,8 @@ def play_games(black_net, white_net, n_games, num_simulations=NUM_SIMULATIONS, t
             visits, _ = eng.search(image, noise=None)   # expand_node + run_mcts, no add_exploration_noise (test.py:37-41)
             a = softmax_sample(visits, temperature, ut)
         else:
-            _, probs, hidden = net.initial(controller_image(hw, hb, t, n, getattr(net, "dtype", torch.float32)))
-            logits = net.policy_logits(hidden) if hasattr(net, "policy_logits") else probs.float().clamp(min=torch.finfo(torch.float32).tiny).log()
+            served = net.initial(controller_image(hw, hb, t, n, getattr(net, "dtype", torch.float32)))
+            logits = net.policy_logits(served[2]) if hasattr(net, "policy_logits") else served[1].float().clamp(min=torch.finfo(torch.float32).tiny).log()
             a = sample_actions(logits, ut, temperature, legal=env.legal)
             a = a.masked_fill(env.done != 0, PASS).to(torch.uint8)   # -1 (a NaN among the logits) is refused as a move; a finished game makes none
         _, status = env.step(a)   # finished games report MZ_ST_DONE and stay untouched

@@ -14,6 +14,7 @@ What is added for the batched engine:
 Return contract (network.py:146-163): ``(value (B,1), policy (B,65) softmaxed, hidden (B,8,8,8))``.
 """
 import copy
+import functools
 
 import torch
 import torch.nn as nn
@@ -90,13 +91,21 @@ class Prediction(nn.Module):
 
 
 @torch.no_grad()
-def policy_logits(prediction, hidden):
+def _policy_logits(prediction, hidden):
     """(n, 65) float32: what the policy head takes the softmax of, from hidden states of any type, in float32 whatever the weights'
     type (the 1x1 convolution as a matrix product).  A probability underflows where a logit does not."""
     ph = prediction.policy_head
     f = lambda t: t.detach().float()  # noqa: E731
     x = torch.relu(f(ph[0].weight).flatten(1) @ hidden.float().flatten(2) + f(ph[0].bias).unsqueeze(1)).flatten(1)
     return F.linear(torch.relu(F.linear(x, f(ph[3].weight), f(ph[3].bias))), f(ph[5].weight), f(ph[5].bias))
+
+
+def policy_logits(net):
+    """that function of hidden states for a network with this module's Prediction.  Others may have heads of another form: AttributeError, so
+    that a property of the same name is not there for them."""
+    if type(getattr(net, "prediction", None)) is not Prediction:
+        raise AttributeError("policy_logits")
+    return functools.partial(_policy_logits, net.prediction)
 
 
 class Network(nn.Module):
@@ -451,9 +460,10 @@ class InferenceEngine:
             return self._infer_x3("repr", image.to(self.dtype))
         return self._finish(self._hidden_initial(image.to(self.dtype)))
 
-    def policy_logits(self, hidden):
-        """the logits behind the policy that initial() / recurrent() returned together with `hidden`"""
-        return policy_logits(self.net.prediction, hidden)
+    @property
+    def policy_logits(self):
+        """policy_logits(hidden): the logits behind the policy that initial() / recurrent() returned together with `hidden`"""
+        return policy_logits(self.net)
 
     @torch.no_grad()
     def recurrent(self, x10, out=None):

@@ -26,7 +26,7 @@ from . import _lib as L
 from . import config
 from .env import BatchedEnv, make_image
 from .mcts import META_ERROR, BatchedMCTS, select_action
-from .network import Network, policy_logits
+from .network import policy_logits
 
 
 class NetworkAdapter:
@@ -35,8 +35,11 @@ class NetworkAdapter:
     def __init__(self, net):
         self.net = net
         self.dtype = torch.float32
-        if isinstance(net, Network):           # others may have heads of another form
-            self.policy_logits = lambda hidden: policy_logits(net.prediction, hidden)
+
+    @property
+    def policy_logits(self):
+        """as InferenceEngine's; networks with heads of another form have none"""
+        return policy_logits(self.net)
 
     @torch.no_grad()
     def initial(self, image):

@@ -113,9 +113,43 @@ def test_logits_are_those_of_the_served_policy(kind):
     _, probs, hidden = engine.initial(image.to(engine.dtype))
     got = engine.policy_logits(hidden)
     assert got.dtype == torch.float32 and got.shape == (n, 65) and not got.requires_grad
-    positive = copy.deepcopy(engine.net.prediction)
+    positive = copy.deepcopy(engine.net)
     for p in positive.parameters():
         p.requires_grad_(False).abs_()
-    size = policy_logits(positive, hidden.abs()).double().amax(1, keepdim=True)       # no term is larger
+    size = policy_logits(positive)(hidden.abs()).double().amax(1, keepdim=True)       # no term is larger
     want = probs.double().log()
     assert bool(((got.double().log_softmax(1) - want).abs() <= 2.0 ** -24 * (2 * 2 * 264 * size + 32 * (1 + want.abs()))).all())
+
+
+def test_adapters_of_other_networks_and_copies_of_adapters():
+    import copy
+    import pickle
+    from muzero_amd.selfplay import NetworkAdapter
+
+    class Other:
+        def initial_inference(self, image):
+            n = image.shape[0]
+            return torch.zeros(n, 1, device="cuda"), torch.full((n, 65), 1.0 / 65, device="cuda"), torch.zeros((n, 8, 8, 8), device="cuda")
+
+    class Changed(torch.nn.Module):
+        def forward(self, hidden):
+            n = hidden.shape[0]
+            return torch.full((n, 65), 1.0 / 65, device="cuda"), torch.zeros(n, 1, device="cuda")
+
+    from muzero_amd import arena
+    from muzero_amd.network import InferenceEngine
+    assert not hasattr(NetworkAdapter(Other()), "policy_logits")
+    arena.play_games(NetworkAdapter(Other()), NetworkAdapter(Other()), 4, num_simulations=0)
+    engine = InferenceEngine(_network(0.0), 4, torch.float32)
+    assert hasattr(engine, "policy_logits")
+    engine.net.prediction = Changed()                       # a head of another form, served by the same engine
+    assert not hasattr(engine, "policy_logits")
+    arena.play_games(engine, engine, 4, num_simulations=0)
+    adapter = NetworkAdapter(_network(0.0).cuda())
+    hidden = torch.rand(3, 8, 8, 8, device="cuda")
+    want = adapter.policy_logits(hidden)
+    for twin in (copy.deepcopy(adapter), pickle.loads(pickle.dumps(adapter))):
+        assert torch.equal(twin.policy_logits(hidden), want)
+        with torch.no_grad():
+            twin.net.prediction.policy_head[-2].bias.add_(1.0)          # its own network, not the first one's
+        assert not torch.equal(twin.policy_logits(hidden), want) and torch.equal(adapter.policy_logits(hidden), want)
