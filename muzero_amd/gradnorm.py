@@ -5,7 +5,7 @@ A list of tensors is one operator: one launch per 256 tensors for the norm and p
 buffer of a ``train.FlatGradBucket`` is a list of one.  Nothing here waits for the GPU.  No CPU fallback: host tensors raise.
 
 Neither has a derivative: where tensors carry a graph of their own and gradients are recorded, a backward pass that comes to the norm
-or to what was scaled raises an error (not under torch.no_grad(), nor for leaves, which are scaled as values, as an optimiser does)."""
+or to what was scaled raises an error.  Not so under torch.no_grad(); and leaves are scaled as values, as an optimiser does."""
 import operator
 import struct
 
@@ -142,4 +142,4 @@ def clip_grad_norm(tensors, max_norm, out=None):
         types = [s | d << 32 for s, d in zip(codes, dst_codes)]
     norm = _call("mz_grad_clip", tensors[0].device, ptrs, dst, sizes, types, index, max_norm)
     torch.autograd.graph.increment_version(outs)      # autograd's check of tensors changed in place sees these too
-    return _NoDerivative.apply(norm, *inner) if inner else norm
+    return _NoDerivative.apply(norm, *recorded) if recorded else norm

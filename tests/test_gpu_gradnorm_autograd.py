@@ -88,3 +88,13 @@ def test_views_that_autograd_takes_nothing_in_place_from():
     with pytest.raises(RuntimeError, match="view"):
         clip_grad_norm(list(torch.split(y, 100)), 0.5)
     assert torch.equal(y.detach(), kept)
+
+
+def test_the_norm_that_clipping_returns_for_leaves():
+    from muzero_amd.gradnorm import clip_grad_norm
+    a, b = _pair()
+    norm = clip_grad_norm([a, b], 1e-2)
+    with pytest.raises(RuntimeError, match="no derivative"):
+        torch.autograd.grad(a.sum() + norm, a)
+    with torch.no_grad():
+        assert not clip_grad_norm([a, b], 1e-2).requires_grad
